@@ -98,17 +98,14 @@ def prepare(case, seed):
   g.manual_seed(int(seed))
   state = dict(case)
   if case["op"] == "clip":
-    types = [DTYPES[case["dtype"] if i % 2 == 0 else case["second"]] for i in range(len(_sizes(case)))]
-    grads, outs, flat = [], [], {}
-    for t in dict.fromkeys(types):
-      flat[t] = torch.empty(sum(s for s, ty in zip(_sizes(case), types) if ty is t), dtype=t, device="cuda")
-    used = dict.fromkeys(flat, 0)
-    for i, (size, t) in enumerate(zip(_sizes(case), types)):
-      x = torch.empty(size, dtype=t, device="cuda").normal_(generator=g)
+    grads, flat = [], {}
+    for i, size in enumerate(_sizes(case)):
+      x = torch.empty(size, dtype=DTYPES[case["dtype"] if i % 2 == 0 else case["second"]], device="cuda").normal_(generator=g)
       grads.append(x.mul_(0.002 * (1 + i % 5)))
-      outs.append(flat[t][used[t]:used[t] + size])   # clipped gradients go to one flat buffer for each type, without gaps
-      used[t] += size
-    state.update(grads=grads, outs=outs, flat=list(flat.values()), groups=[[x for x in grads if x.dtype is t] for t in flat])
+      flat[x.dtype] = flat.get(x.dtype, 0) + size
+    # clipped gradients go to one flat buffer for each type, without gaps
+    state.update(grads=grads, flat=[torch.empty(size, dtype=t, device="cuda") for t, size in flat.items()],
+                 groups=[[x for x in grads if x.dtype is t] for t in flat])
     return state
   state["ids"] = _ids(case, g)
   t = DTYPES[case["dtype"]]
@@ -162,8 +159,7 @@ def _rows(s):
 def _clip(s):
   if own:
     from orca_amd import ops
-    norm = ops.clip_grad_norm(s["grads"], s["max_norm"], out=s["outs"])
-    return norm, s["flat"]
+    return ops.clip_grad_norm(s["grads"], s["max_norm"], flat=s["flat"]), s["flat"]
   flat = [torch.cat(x) for x in s["groups"]]
   norm = torch.stack([x.float().square().sum() for x in flat]).sum().sqrt()
   c = (s["max_norm"] / (norm + 1e-6)).clamp(max=1.0)
