@@ -35,6 +35,11 @@ extern "C" {
 #define ORCA_MAX_K 20       /* most neighbours per query in orca_tgat_forward */
 #define ORCA_MAX_WORLD 64   /* most ranks of an owner-computes step (orca_engine_desc) */
 
+/* element types of the entry points that take more than fp32 */
+#define ORCA_F32 0
+#define ORCA_BF16 1
+#define ORCA_F16 2
+
 #define ORCA_OK 0
 #define ORCA_EINVAL -1      /* bad argument (ValueError / assert upstream) */
 #define ORCA_EHIP -2        /* HIP runtime failure */
@@ -408,6 +413,54 @@ int64_t orca_decoder_train_workspace_floats(int64_t bs);
 int orca_decoder_train(const float* emb, int64_t bs, const float* fc1_w, const float* fc1_b, const float* fc2_w,
                        const float* fc2_b, float* loss, float* prob, float* d_emb, float* g_fc1_w, float* g_fc1_b,
                        float* g_fc2_w, float* g_fc2_b, float* workspace, void* stream);
+
+/* ---- embedding tables with gradients (not in the reference, whose tables are data) ----------------------------- */
+
+/* out[p, :] = scale * table[ids[p], :], computed in fp32 and rounded once to the table's type (ORCA_F32 / BF16 / F16).
+ * table [n_rows, width] with rows `ld` elements apart, ids int64 or int32 (exactly one list non-null), out [n, width]
+ * without gaps.  An id outside [0, n_rows) reads as a row of zeros.  No alignment beyond the element's is needed;
+ * 1 <= width <= 65536. */
+int orca_embedding_forward(const void* table, int dtype, int64_t n_rows, int64_t width, int64_t ld, const int64_t* idx64,
+                           const int32_t* idx32, int64_t n, float scale, void* out, void* stream);
+/* The gradient of that lookup for the table: grad_table[v, :] = scale * sum over {p : ids[p] = v} of grad_out[p, :], zeros
+ * for a v without an occurrence; accumulate != 0: the sums are added to what is there and the other rows are left alone.
+ * Ids outside [0, num_rows) and the id padding_idx (negative: none) contribute nothing; their rows of grad_out are never
+ * used.  grad_out [n, width] with rows ld_grad elements apart (0: every row is the same one); grad_table's rows lie
+ * ld_table >= width elements apart, its type is grad_dtype or ORCA_F32.  Sums are fp32 in an order that (id, position)
+ * alone decides (the positions are sorted by id): the same call gives the same bits.  n and num_rows under 2^31 - 1.
+ * workspace: orca_embedding_backward_workspace_bytes(n, width, num_rows) bytes (-1: unsupported sizes), 16-byte aligned,
+ * contents irrelevant. */
+int64_t orca_embedding_backward_workspace_bytes(int64_t n, int64_t width, int64_t num_rows);
+int orca_embedding_backward(const void* grad_out, int grad_dtype, int64_t ld_grad, const int64_t* idx64, const int32_t* idx32,
+                            int64_t n, int64_t width, int64_t num_rows, int64_t padding_idx, float scale, int accumulate,
+                            void* grad_table, int table_dtype, int64_t ld_table, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+/* The same gradient row-sparse: ids[0 .. *count) = the distinct ids that contribute, ascending, rows[r, :] = the gradient
+ * of ids[r] (type rows_dtype: grad_dtype or ORCA_F32), *count (device int) their number.  ids and rows have room for n;
+ * what lies behind *count is left as it was. */
+int orca_embedding_backward_rows(const void* grad_out, int grad_dtype, int64_t ld_grad, const int64_t* idx64,
+                                 const int32_t* idx32, int64_t n, int64_t width, int64_t num_rows, int64_t padding_idx,
+                                 float scale, int64_t* ids, void* rows, int rows_dtype, int32_t* count, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
+/* ---- gradient norm and clipping (torch.nn.utils.clip_grad_norm_; not called by the reference) ------------------- */
+
+/* Tensor i of the list: sizes[i] elements of type dtypes[i] (ORCA_F32 / BF16 / F16) at grads[i], in any order in memory
+ * but without gaps.  rows (NULL: none is row-sparse): rows[i] != NULL is a device count, and only the first
+ * *rows[i] * widths[i] elements (at most sizes[i]) are there.  All arrays are HOST arrays of length n.
+ * *norm = sqrt(sum of squares over all tensors), squares and sums in fp64 in an order the sizes alone decide;
+ * *coef (may be NULL) = min(1, max_norm / (sqrt(..) + 1e-6)), NaN if the norm is; norm, coef: device floats.
+ * workspace: orca_grad_norm_workspace_bytes() bytes, 8-byte aligned, contents irrelevant. */
+int64_t orca_grad_norm_workspace_bytes(void);
+int orca_grad_norm(int n, void* const* grads, const int64_t* sizes, const uint8_t* dtypes, const int32_t* const* rows,
+                   const int32_t* widths, double max_norm, float* norm, float* coef, void* workspace, void* stream);
+/* The norm, and every gradient multiplied by that coefficient (in fp32, rounded once to its type): in place when
+ * flat == NULL (a coefficient of 1 then writes nothing), else flat[dtype] (HOST array of three device pointers) receives the
+ * products of the gradients of that type one after another without gaps, in the list's order; flat buffers need no
+ * alignment beyond the element's and must not overlap the gradients.  What lies behind the last row of a row-sparse
+ * gradient is left as it was, in its part of flat[] too. */
+int orca_clip_grads(int n, void* const* grads, const int64_t* sizes, const uint8_t* dtypes, const int32_t* const* rows,
+                    const int32_t* widths, double max_norm, void* const* flat, float* norm, void* workspace, void* stream);
 
 /* optimizer.step() of train.py:238 for torch.optim.Adam(tgn.parameters(), lr) (train.py:180; no weight decay, no
  * amsgrad) over n tensors in one launch per 24 tensors: params / grads / exp_avg / exp_avg_sq and sizes are HOST arrays

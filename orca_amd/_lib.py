@@ -10,6 +10,7 @@ LIB_PATH = os.environ.get("ORCA_HIP_LIB") or os.path.join(_HERE, "liborca_hip.so
 ORCA_D = 100
 ORCA_MAX_DE = 192
 ORCA_MAX_K = 20
+ORCA_F32, ORCA_BF16, ORCA_F16 = 0, 1, 2
 MAX_WORLD = 64      # ORCA_MAX_WORLD
 
 vp = ctypes.c_void_p
@@ -116,6 +117,13 @@ SIGNATURES = {
     "orca_decoder_train_workspace_floats": (i64, [i64]),
     "orca_decoder_train": (i32, [vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "orca_adam_step": (i32, [i32, vp, vp, vp, vp, vp, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, i64, vp]),
+    "orca_embedding_forward": (i32, [vp, i32, i64, i64, i64, vp, vp, i64, ctypes.c_float, vp, vp]),
+    "orca_embedding_backward_workspace_bytes": (i64, [i64, i64, i64]),
+    "orca_embedding_backward": (i32, [vp, i32, i64, vp, vp, i64, i64, i64, i64, ctypes.c_float, i32, vp, i32, i64, vp, i64, vp]),
+    "orca_embedding_backward_rows": (i32, [vp, i32, i64, vp, vp, i64, i64, i64, i64, ctypes.c_float, vp, vp, i32, vp, vp, i64, vp]),
+    "orca_grad_norm_workspace_bytes": (i64, []),
+    "orca_grad_norm": (i32, [i32, vp, vp, vp, vp, vp, ctypes.c_double, vp, vp, vp, vp]),
+    "orca_clip_grads": (i32, [i32, vp, vp, vp, vp, vp, ctypes.c_double, vp, vp, vp, vp]),
     "orca_find_uncached": (i32, [vp, i64, vp, i64, vp, vp, i64, i64, vp, vp, i64, vp, vp]),
     "orca_engine_create": (i32, [ctypes.POINTER(EngineDesc), ctypes.POINTER(vp)]),
     "orca_engine_destroy": (i32, [vp]),

@@ -8,9 +8,14 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "liborca_hip.so")
-SOURCES = ["csr.hip", "tgat.hip", "tgat_bwd.hip", "gru_bwd.hip", "gru.hip", "state.hip", "plan.hip", "plan_dev.hip", "engine.hip", "optim.hip", "decoder.hip"]
+SOURCES = ["csr.hip", "tgat.hip", "tgat_bwd.hip", "gru_bwd.hip", "gru.hip", "state.hip", "plan.hip", "plan_dev.hip", "engine.hip", "optim.hip", "clip.hip", "embedding.hip", "decoder.hip"]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-Wall",
          "-Wno-unused-result", "-Wno-unused-function"]
+
+
+# no packed fp32 instructions in the sources that carry this (some of their forms have given wrong results on gfx950)
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SCALAR_FP32 = {"clip.hip", "embedding.hip"}
 
 
 def _stale(target, deps):
@@ -33,7 +38,7 @@ def build(force=False, verbose=False):
     obj = os.path.join(CSRC, "build", s.replace(".hip", ".o"))
     objs.append(obj)
     if force or _stale(obj, [src] + headers):
-      jobs.append([hipcc] + FLAGS + ["-c", src, "-o", obj])
+      jobs.append([hipcc] + FLAGS + (NO_PACKED if s in SCALAR_FP32 else []) + ["-c", src, "-o", obj])
 
   def run(cmd):
     if verbose:

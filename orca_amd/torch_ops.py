@@ -7,6 +7,7 @@ the reference's training loop differentiates (train.py:225-226 loss.backward()):
                       encodings of :126,132 fused in (rows fetched by index from the feature tables)
   orca::gru_cell      nn.GRUCell of modules/memory_updater.py:86 (get_updated_memory :56-78 applies it to the rows
                       of the pending ids a batch reads and keeps them in the graph)
+  orca::embedding     a learned table's rows by id, scaled (no counterpart upstream, where every table is data)
   orca::message_store / orca::history_push / orca::history_pull     state writes and reads that are detached
                       upstream (tgn_model.py:172-191, history.py:32-40 run under no_grad)
 
@@ -223,5 +224,26 @@ def _hpp_backward(ctx, g_out):
 _lib.register_autograd("orca::history_pull_pushed", _hpp_backward, setup_context=_hpp_setup)
 
 
+# ---- a learned table: lookup with its gradient ------------------------------------------------------------------
+@_lib.custom_op("orca::embedding", mutates_args=())
+def embedding(table: Tensor, ids: Tensor, scale: float, padding_idx: int) -> Tensor:
+  """scale * table[ids]; the row of padding_idx (negative: none) reads like any other and gets no gradient"""
+  return ops.embedding(table, ids, scale)
+
+
+def _embedding_setup(ctx, inputs, output):
+  table, ids, ctx.scale, ctx.padding_idx = inputs
+  ctx.num_rows = table.shape[0]
+  ctx.save_for_backward(ids)
+
+
+def _embedding_backward(ctx, g_out):
+  ids, = ctx.saved_tensors
+  return ops.embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx), None, None, None
+
+
+_lib.register_autograd("orca::embedding", _embedding_backward, setup_context=_embedding_setup)
+
+
 OPS = ("sample_recent", "sample_uniform", "tgat_dense", "tgat_gather", "gru_cell", "message_store", "history_push",
-       "history_pull", "history_pull_pushed")
+       "history_pull", "history_pull_pushed", "embedding")
