@@ -93,14 +93,43 @@ int embedding_typed(const void* table, int64_t n_rows, int64_t width, int64_t ld
                : launch_embedding<T, 1>(table, n_rows, width, ld, idx32, n, scale, out, stream);
 }
 
+// ---- zeros ahead of the sums -----------------------------------------------------------------------------------------
+// A dense gradient starts as zeros; nothing before the sums reads it, so the launches of the sort carry the zero fill in extra
+// workgroups: the sort waits on latency with a few dozen workgroups, the fill on the HBM, and the longer of the two is what counts.
+constexpr int FILL_PIECE = 32768;       // bytes a workgroup writes at a time
+struct fill_job {
+  char* p;                      // `rows` rows of `bytes` bytes, `pitch` bytes apart (a table without gaps is one row)
+  int64_t bytes, pitch, per_row, from, to;      // pieces of a row; this launch's pieces
+};
+template <int THREADS> __device__ __forceinline__ void fill_pieces(const fill_job& f, int64_t block, int64_t blocks) {
+  const u32x4 zero = {0, 0, 0, 0};
+  for (int64_t i = f.from + block; i < f.to; i += blocks) {
+    const int64_t r = i / f.per_row, at = (i - r * f.per_row) * FILL_PIECE;
+    char* p = f.p + r * f.pitch + at;
+    const int len = (int)(f.bytes - at < FILL_PIECE ? f.bytes - at : FILL_PIECE);
+#pragma unroll
+    for (int k = 0; k < FILL_PIECE / (16 * THREADS); ++k) {
+      const int b = ((int)threadIdx.x + THREADS * k) * 16;
+      if (b + 16 <= len) {
+        store16(p + b, zero);
+      } else {
+        for (int e = b; e < len; e += 2) *reinterpret_cast<uint16_t*>(p + e) = 0;
+      }
+    }
+  }
+}
+__global__ __launch_bounds__(512) void k_fill(fill_job f) { fill_pieces<512>(f, blockIdx.x, gridDim.x); }
+
 // ---- sort of the positions by id -------------------------------------------------------------------------------------
 // Stable least-significant-digit radix sort of (key, position) pairs; key = the id, or num_rows for what has no row (the padding
 // id, ids outside the table): those end up last and are dropped.  A tile is SORT_TILE consecutive pairs of one workgroup; within it
 // a wave owns 64 * SORT_ITEMS consecutive pairs and ranks them 64 at a time: the lanes with the same digit find each other with one
-// ballot per digit bit.
+// ballot per digit bit.  Two launches per pass (count, scatter); with many tiles a third one adds the counts up.
 constexpr int SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS;
-constexpr int MAX_DIGIT = 11, MAX_BINS = 1 << MAX_DIGIT;
+constexpr int MIN_DIGIT = 2, MAX_DIGIT = 11, MAX_BINS = 1 << MAX_DIGIT;
+constexpr int DIRECT_TILES = 64;        // up to this many tiles every workgroup adds the counts up itself
 static_assert(SORT_TILE <= 65536, "16-bit counts within a tile");
+static_assert(MAX_BINS == 4 * SORT_THREADS, "a thread takes four neighbouring bins");
 struct pair32 { uint32_t pos, key; };
 
 struct sort_src {               // where a pass reads: the caller's ids (first pass) or the pairs of the pass before
@@ -117,16 +146,24 @@ __device__ __forceinline__ pair32 sort_read(const sort_src& s, int64_t i) {
 }
 
 // counts[tile][bin] of this pass' digit
-__global__ __launch_bounds__(SORT_THREADS) void k_sort_count(sort_src src, int shift, int bins, uint32_t* __restrict__ counts) {
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_count(sort_src src, int shift, int bins, uint32_t* __restrict__ counts, int tiles, fill_job fill) {
   __shared__ uint32_t h[MAX_BINS];
-  for (int b = threadIdx.x; b < bins; b += SORT_THREADS) h[b] = 0;
-  __syncthreads();
+  if ((int)blockIdx.x >= tiles) {
+    fill_pieces<SORT_THREADS>(fill, (int)blockIdx.x - tiles, (int)gridDim.x - tiles);
+    return;
+  }
+  pair32 p[SORT_ITEMS];
   const int64_t base = (int64_t)blockIdx.x * SORT_TILE;
 #pragma unroll
   for (int u = 0; u < SORT_ITEMS; ++u) {
     const int64_t i = base + threadIdx.x + SORT_THREADS * u;
-    if (i < src.n) atomicAdd(&h[(sort_read(src, i).key >> shift) & (bins - 1)], 1u);
+    p[u] = i < src.n ? sort_read(src, i) : pair32{0u, 0u};
   }
+  for (int b = threadIdx.x; b < bins; b += SORT_THREADS) h[b] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < SORT_ITEMS; ++u)
+    if (base + threadIdx.x + SORT_THREADS * u < src.n) atomicAdd(&h[(p[u].key >> shift) & (bins - 1)], 1u);
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += SORT_THREADS) counts[(int64_t)blockIdx.x * bins + b] = h[b];
 }
@@ -158,61 +195,82 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v, int lane) {
   return v;
 }
 
+// the lanes of `in` whose digit equals this lane's
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, int digit_bits, bool in) {
+  uint64_t peers = __ballot(in);
+  for (int k = 0; k < digit_bits; ++k) {
+    const uint64_t m = __ballot((d >> k) & 1);
+    peers &= (d >> k) & 1 ? m : ~m;
+  }
+  return peers;
+}
+
+// totals == null: counts holds every tile's counts, which this workgroup adds up itself
 __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int shift, int digit_bits, const uint32_t* __restrict__ counts,
-                                                               const uint32_t* __restrict__ totals, pair32* __restrict__ out) {
+                                                               const uint32_t* __restrict__ totals, pair32* __restrict__ out, int tiles, fill_job fill) {
   __shared__ uint32_t place[MAX_BINS];                   // where the tile's first pair of a digit goes
   __shared__ uint16_t part[SORT_WAVES][MAX_BINS];        // the wave's counts of a digit, then those of the waves before it
   __shared__ uint32_t wave_sum[SORT_WAVES];
+  if ((int)blockIdx.x >= tiles) {
+    fill_pieces<SORT_THREADS>(fill, (int)blockIdx.x - tiles, (int)gridDim.x - tiles);
+    return;
+  }
   const int bins = 1 << digit_bits, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  for (int b = t; b < bins; b += SORT_THREADS)
-#pragma unroll
-    for (int w = 0; w < SORT_WAVES; ++w) part[w][b] = 0;
-  __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * SORT_TILE + wave * (64 * SORT_ITEMS);
   pair32 p[SORT_ITEMS];
-  uint32_t rank[SORT_ITEMS];
 #pragma unroll
   for (int u = 0; u < SORT_ITEMS; ++u) {
     const int64_t i = base + 64 * u + lane;
     p[u] = i < src.n ? sort_read(src, i) : pair32{0u, 0u};
   }
+  // the thread's four bins: pairs of them in the tiles before this one, and in all
+  u32x4 before = {0, 0, 0, 0}, total = {0, 0, 0, 0};
+  if (4 * t < bins) {
+    if (totals) {
+      before = load16(counts + (int64_t)blockIdx.x * bins + 4 * t);
+      total = load16(totals + 4 * t);
+    } else {
+      for (int k0 = 0; k0 < tiles; k0 += 8) {
+        u32x4 c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) c[u] = k0 + u < tiles ? load16(counts + (int64_t)(k0 + u) * bins + 4 * t) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (k0 + u < (int)blockIdx.x) before += c[u];
+          total += c[u];
+        }
+      }
+    }
+  }
+  for (int k = t; k < SORT_WAVES * MAX_BINS / 8; k += SORT_THREADS) reinterpret_cast<u32x4*>(&part[0][0])[k] = u32x4{0, 0, 0, 0};
+  __syncthreads();
+  uint32_t rank[SORT_ITEMS];
 #pragma unroll
   for (int u = 0; u < SORT_ITEMS; ++u) {
     const bool in = base + 64 * u + lane < src.n;
     const uint32_t d = (p[u].key >> shift) & (uint32_t)(bins - 1);
-    uint64_t peers = __ballot(in);
-    for (int k = 0; k < digit_bits; ++k) {
-      const uint64_t m = __ballot((d >> k) & 1);
-      peers &= (d >> k) & 1 ? m : ~m;
-    }
+    const uint64_t peers = same_digit(d, digit_bits, in);
     const int leader = in ? __ffsll((unsigned long long)peers) - 1 : lane;
-    uint32_t before = 0;
+    uint32_t seen = 0;
     if (in && lane == leader) {          // (one lane per digit, and the counts are the wave's own)
-      before = part[wave][d];
-      part[wave][d] = (uint16_t)(before + (uint32_t)__popcll(peers));
+      seen = part[wave][d];
+      part[wave][d] = (uint16_t)(seen + (uint32_t)__popcll(peers));
     }
-    before = __shfl(before, leader);
-    rank[u] = before + (uint32_t)__popcll(peers & ((1ULL << lane) - 1));
+    rank[u] = __shfl(seen, leader) + (uint32_t)__popcll(peers & ((1ULL << lane) - 1));
   }
-  // exclusive prefix of totals over the bins: a thread takes MAX_BINS / SORT_THREADS neighbouring bins
-  constexpr int PER = MAX_BINS / SORT_THREADS;
-  uint32_t tot[PER], mine = 0;
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int b = t * PER + k;
-    tot[k] = b < bins ? totals[b] : 0u;
-    mine += tot[k];
-  }
+  // exclusive prefix of the totals over the bins
+  const uint32_t mine = total[0] + total[1] + total[2] + total[3];
   const uint32_t inc = wave_inclusive(mine, lane);
   if (lane == 63) wave_sum[wave] = inc;
   __syncthreads();
   uint32_t run = inc - mine;
   for (int w = 0; w < wave; ++w) run += wave_sum[w];
+  if (4 * t < bins) {
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int b = t * PER + k;
-    if (b < bins) {
-      place[b] = run + counts[(int64_t)blockIdx.x * bins + b];
+    for (int k = 0; k < 4; ++k) {
+      const int b = 4 * t + k;
+      place[b] = run + before[k];
+      run += total[k];
       uint32_t sum = 0;
 #pragma unroll
       for (int w = 0; w < SORT_WAVES; ++w) {
@@ -221,15 +279,15 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
         sum += c;
       }
     }
-    run += tot[k];
   }
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u)
+  for (int u = 0; u < SORT_ITEMS; ++u) {
     if (base + 64 * u + lane < src.n) {
       const uint32_t d = (p[u].key >> shift) & (uint32_t)(bins - 1);
       out[place[d] + part[wave][d] + rank[u]] = p[u];
     }
+  }
 }
 
 // ---- the rows' numbers (row-sparse form) -----------------------------------------------------------------------------
@@ -292,7 +350,12 @@ __global__ __launch_bounds__(SORT_THREADS) void k_rank(const pair32* __restrict_
 }
 
 // ---- sums over the windows of the sorted list ------------------------------------------------------------------------
-constexpr int WINDOW = 32;        // sorted pairs per team
+// The sorted list is cut into windows of `window` pairs.  A team of 2^log_l lanes (a lane holds one 16-byte chunk of the columns; a
+// whole workgroup for rows of 4 KB, so that the pieces of a row are requested together: in column blocks far apart in the grid the
+// rows' first KBs met a quarter of the HBM channels at a time) walks one window in order.  A run of equal ids that lies inside the
+// window is written out; one that crosses a border leaves its sum in `part` for k_segment_join.
+constexpr int SEG_PAIRS = 2048;   // pairs of one workgroup's windows, at most
+constexpr int SEG_U = 8;          // rows requested together; the next ones are on their way while these are added
 struct seg_args {
   const void* g;                  // [n, width], row stride ld_g (0: every row is the same one)
   int64_t ld_g, n, ld_out;
@@ -300,26 +363,51 @@ struct seg_args {
   const uint32_t* rank;           // or null: a row's place in the output is its id
   void* out;
   float* part;                    // [2 * windows, width]: what a window adds to a run that began before it / that it begins and does not end
-  int width, chunks, log_l, accumulate;
+  int width, chunks, log_l, window, col_blocks;
   uint32_t none;
   float scale;
 };
 
-// A team of 2^log_l lanes walks one window of the sorted list in order, a lane holding one 16-byte chunk of the columns.  A run of
-// equal ids that lies inside the window is written out; one that crosses a border leaves its sum in `part` for k_segment_join.
-template <class TI, class TO, int VEC>
+template <int VEC, class T> struct raw_chunk {        // a chunk as it was loaded
+  u32x4 r;
+  __device__ __forceinline__ void load(const T* p) { r = load16(p); }
+  __device__ __forceinline__ void add_to(float (&acc)[VEC]) const {
+    float f[VEC];
+    unpack16<T>(r, f);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] += f[j];
+  }
+};
+template <class T> struct raw_chunk<1, T> {
+  T r;
+  __device__ __forceinline__ void load(const T* p) { r = *p; }
+  __device__ __forceinline__ void add_to(float (&acc)[1]) const { acc[0] += (float)r; }
+};
+
+template <class TI, class TO, int VEC, bool ACCUMULATE>
 __global__ __launch_bounds__(256) void k_segment_sum(seg_args a) {
-  const int team = threadIdx.x >> a.log_l, tl = threadIdx.x & ((1 << a.log_l) - 1);
-  const int64_t w = (int64_t)blockIdx.x * (256 >> a.log_l) + team;
-  const int c = ((int)blockIdx.y << a.log_l) + tl;
-  const int64_t i0 = w * WINDOW;
-  if (i0 >= a.n || c >= a.chunks) return;
-  const int64_t i1 = i0 + WINDOW < a.n ? i0 + WINDOW : a.n;
+  __shared__ pair32 list[SEG_PAIRS + 2];        // [k + 1] = pair k of the workgroup's windows; its neighbours at both ends
+  __shared__ uint32_t row[SEG_PAIRS];           // [k] = the output row of pair k (row-sparse form)
+  const int teams = 256 >> a.log_l, team = threadIdx.x >> a.log_l, tl = threadIdx.x & ((1 << a.log_l) - 1);
+  const int64_t w0 = (int64_t)(blockIdx.x / (uint32_t)a.col_blocks) * teams;
+  const int c = ((int)(blockIdx.x % (uint32_t)a.col_blocks) << a.log_l) + tl;
+  const int64_t base = w0 * a.window;
+  const int count = (int)(a.n - base < teams * a.window ? a.n - base : teams * a.window);
+  for (int k = threadIdx.x; k < count + 2; k += 256) {
+    const int64_t i = base - 1 + k;
+    list[k] = i >= 0 && i < a.n ? a.s[i] : pair32{0u, ~0u};          // (~0u: no key)
+  }
+  if (a.rank)       // (ahead of the loop: a load inside it would wait for the rows on their way)
+    for (int k = threadIdx.x; k < count; k += 256) row[k] = a.rank[base + k];
+  __syncthreads();
+  const int first = team * a.window, last = min(first + a.window, count);
+  if (first >= count || c >= a.chunks || list[first + 1].key == a.none) return;
+  const int64_t w = w0 + team;
   const int col = VEC == 1 ? c : min(c * VEC, a.width - VEC), own = c * VEC - col;      // (elements before `own` are the neighbour's)
   const TI* g = (const TI*)a.g + col;
-  uint32_t cur = a.s[i0].key;
-  bool head = i0 > 0 && a.s[i0 - 1].key == cur;
-  int64_t first = i0;             // first pair of the current run in this window
+  uint32_t cur = list[first + 1].key;
+  bool head = list[first].key == cur;
+  int begin = first;              // first pair of the current run in this window
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
@@ -329,12 +417,12 @@ __global__ __launch_bounds__(256) void k_segment_sum(seg_args a) {
       store_chunk<VEC, float>(a.part + (2 * w + (head ? 0 : 1)) * a.width + col, acc);
       return;
     }
-    const int64_t r = a.rank ? (int64_t)a.rank[first] : (int64_t)cur;
+    const int64_t r = a.rank ? row[begin] : cur;
     TO* o = (TO*)a.out + r * a.ld_out + col;
     float f[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) f[j] = acc[j] * a.scale;
-    if (a.accumulate) {
+    if constexpr (ACCUMULATE) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
         if (j >= own) o[j] = (TO)((float)o[j] + f[j]);
@@ -342,93 +430,128 @@ __global__ __launch_bounds__(256) void k_segment_sum(seg_args a) {
       store_chunk<VEC, TO>(o, f);
     }
   };
-  constexpr int U = 8;
-  for (int64_t i = i0; i < i1 && cur != a.none; i += U) {
-    pair32 p[U];
-    float v[U][VEC];
+  typedef raw_chunk<VEC, TI> raw;
+  auto request = [&](raw (&v)[SEG_U], int k) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) p[u] = a.s[i + u < i1 ? i + u : i1 - 1];
+    for (int u = 0; u < SEG_U; ++u) v[u].load(g + (int64_t)list[min(k + u, last - 1) + 1].pos * a.ld_g);
+  };
+  auto add = [&](const raw (&v)[SEG_U], int k) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_chunk<VEC, TI>(g + (int64_t)p[u].pos * a.ld_g, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u >= i1) break;
-      if (p[u].key != cur) {
+    for (int u = 0; u < SEG_U; ++u) {
+      if (k + u >= last) break;
+      const uint32_t key = list[k + u + 1].key;
+      if (key != cur) {
         flush(false);
-        cur = p[u].key;
+        cur = key;
         head = false;
-        first = i + u;
+        begin = k + u;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j] += v[u][j];
+      v[u].add_to(acc);
     }
+  };
+  raw va[SEG_U], vb[SEG_U];
+  request(va, first);
+  for (int k = first; k < last; k += 2 * SEG_U) {
+    if (k + SEG_U < last) request(vb, k + SEG_U);
+    add(va, k);
+    if (k + SEG_U >= last) break;
+    if (k + 2 * SEG_U < last) request(va, k + 2 * SEG_U);
+    add(vb, k + SEG_U);
   }
-  flush(i1 < a.n && a.s[i1].key == cur);
+  flush(list[last + 1].key == cur);
 }
 
-// The runs that cross window borders: a workgroup takes the run that window blockIdx.x begins and does not end, its teams each a
-// consecutive share of the windows' sums; the shares are added in the windows' order.
-template <class TO>
+// The runs that cross window borders, each taken by the window that begins it: sum of what that window and the following ones left in
+// `part`, in their order.  A team takes one window; a run over more than JOIN_SHORT windows is left to the whole workgroup, whose teams
+// take a consecutive share of the terms each.
+constexpr int JOIN_SHORT = 16;
+template <class TO, bool ACCUMULATE>
 __global__ __launch_bounds__(256) void k_segment_join(seg_args a) {
   __shared__ float4 share[256];
-  const int64_t w = blockIdx.x, i0 = w * WINDOW, i1 = i0 + WINDOW;
-  if (i1 >= a.n) return;
-  const uint32_t key = a.s[i1 - 1].key;
-  if (key == a.none || a.s[i1].key != key || (i0 > 0 && a.s[i0 - 1].key == key)) return;      // (workgroup-uniform)
-  int64_t terms = 1;              // the window's own sum, and one of each window that begins inside the run
-  for (;;) {
-    const int64_t f = (w + terms + threadIdx.x) * WINDOW;
-    const int m = __syncthreads_count(f < a.n && a.s[f].key == key);
-    terms += m;
-    if (m < 256) break;
-  }
+  __shared__ int64_t queue[256];
+  __shared__ int queued;
   const int lanes = 1 << a.log_l, teams = 256 >> a.log_l, team = threadIdx.x >> a.log_l, tl = threadIdx.x & (lanes - 1);
-  const int col = (((int)blockIdx.y << a.log_l) + tl) * 4;
+  const int64_t w = (int64_t)(blockIdx.x / (uint32_t)a.col_blocks) * teams + team;
+  const int col = (((int)(blockIdx.x % (uint32_t)a.col_blocks) << a.log_l) + tl) * 4;
   const int have = col >= a.width ? 0 : min(4, a.width - col);
-  const int64_t each = ceil_div64(terms, teams), b = team * each, e = b + each < terms ? b + each : terms;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto term = [&](int64_t k) {
+  if (threadIdx.x == 0) queued = 0;
+  __syncthreads();
+  auto term = [&](int64_t w, int64_t k) {         // k = 0: the beginning window's own sum
     const float* q = a.part + (k == 0 ? 2 * w + 1 : 2 * (w + k)) * a.width + col;
-    float4 v;
-    v.x = have > 0 ? q[0] : 0.f;
-    v.y = have > 1 ? q[1] : 0.f;
-    v.z = have > 2 ? q[2] : 0.f;
-    v.w = have > 3 ? q[3] : 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (have == 4) {
+      const u32x4 r = load16(q);
+      __builtin_memcpy(&v, &r, 16);
+    } else {
+      if (have > 0) v.x = q[0];
+      if (have > 1) v.y = q[1];
+      if (have > 2) v.z = q[2];
+    }
     return v;
   };
-  for (int64_t k = b; k < e; k += 8) {
-    float4 v[8];
+  auto sum = [&](int64_t w, int64_t b, int64_t e) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t k = b; k < e; k += 8) {
+      float4 v[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = k + u < e ? term(k + u) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int u = 0; u < 8; ++u) v[u] = k + u < e ? term(w, k + u) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) { acc.x += v[u].x; acc.y += v[u].y; acc.z += v[u].z; acc.w += v[u].w; }
-  }
-  share[threadIdx.x] = acc;
-  __syncthreads();
-  if (team != 0 || have == 0) return;
-  for (int q = 1; q < teams; ++q) {
-    const float4 v = share[(q << a.log_l) + tl];
-    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-  }
-  const int64_t r = a.rank ? (int64_t)a.rank[i1 - 1] : (int64_t)key;
-  TO* o = (TO*)a.out + r * a.ld_out + col;
-  const float f[4] = {acc.x * a.scale, acc.y * a.scale, acc.z * a.scale, acc.w * a.scale};
-  for (int j = 0; j < have; ++j) o[j] = (TO)(a.accumulate ? (float)o[j] + f[j] : f[j]);
-}
-
-// zeros over the rows of a table (rows of `bytes` bytes, `pitch` bytes apart; a table without gaps is one row)
-__global__ __launch_bounds__(256) void k_zero_rows(char* __restrict__ out, int64_t rows, int64_t bytes, int64_t pitch) {
-  const int64_t per = ceil_div64(bytes, 16), total = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = rows == 1 ? 0 : i / per, b = (i - r * per) * 16;
-    char* p = out + r * pitch + b;
-    if (b + 16 <= bytes) {
-      store16(p, u32x4{0, 0, 0, 0});
-    } else {
-      for (int64_t k = b; k < bytes; k += 2) *reinterpret_cast<uint16_t*>(out + r * pitch + k) = 0;
+      for (int u = 0; u < 8; ++u) { acc.x += v[u].x; acc.y += v[u].y; acc.z += v[u].z; acc.w += v[u].w; }
     }
+    return acc;
+  };
+  auto write = [&](int64_t w, uint32_t key, float4 acc) {
+    const int64_t r = a.rank ? (int64_t)a.rank[(w + 1) * a.window - 1] : (int64_t)key;
+    TO* o = (TO*)a.out + r * a.ld_out + col;
+    const float f[4] = {acc.x * a.scale, acc.y * a.scale, acc.z * a.scale, acc.w * a.scale};
+    for (int j = 0; j < have; ++j) o[j] = (TO)(ACCUMULATE ? (float)o[j] + f[j] : f[j]);
+  };
+  const int64_t i0 = w * a.window, i1 = i0 + a.window;
+  if (i1 < a.n) {
+    const uint32_t key = a.s[i1 - 1].key;
+    if (key != a.none && a.s[i1].key == key && !(i0 > 0 && a.s[i0 - 1].key == key)) {       // (the same in the team's lanes)
+      int terms = 1;
+      for (int t0 = 1; t0 <= JOIN_SHORT; t0 += lanes) {
+        const int64_t f = (w + t0 + tl) * a.window;
+        const uint64_t m = __ballot(f < a.n && a.s[f].key == key);
+        const uint64_t of_team = lanes == 64 ? m : (m >> (threadIdx.x & 63 & ~(lanes - 1))) & ((1ULL << lanes) - 1);
+        const int in = __popcll(of_team);
+        terms += in;
+        if (in < lanes) break;
+      }
+      if (terms <= JOIN_SHORT) {
+        write(w, key, sum(w, 0, terms));
+      } else if (tl == 0) {
+        queue[atomicAdd(&queued, 1)] = w;
+      }
+    }
+  }
+  __syncthreads();
+  const int todo = queued;
+  for (int q = 0; q < todo; ++q) {                // (the order of the queue does not matter: its runs are independent)
+    const int64_t w = queue[q];
+    const uint32_t key = a.s[(w + 1) * a.window - 1].key;
+    int64_t terms = 1;
+    for (;;) {
+      const int64_t f = (w + terms + threadIdx.x) * a.window;
+      const int m = __syncthreads_count(f < a.n && a.s[f].key == key);
+      terms += m;
+      if (m < 256) break;
+    }
+    const int64_t each = ceil_div64(terms, teams), b = team * each, e = b + each < terms ? b + each : terms;
+    share[threadIdx.x] = sum(w, b, e);
+    __syncthreads();
+    if (team == 0 && have) {
+      float4 acc = share[tl];
+      for (int t = 1; t < teams; ++t) {
+        const float4 v = share[(t << a.log_l) + tl];
+        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+      }
+      write(w, key, acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -439,9 +562,24 @@ sort_plan plan_sort(int64_t n, int64_t num_rows) {
   while (bits < 32 && (num_rows >> bits) != 0) ++bits;        // keys 0 .. num_rows
   sort_plan s;
   s.passes = (bits + MAX_DIGIT - 1) / MAX_DIGIT;
-  s.digit = (bits + s.passes - 1) / s.passes;
+  s.digit = std::max(MIN_DIGIT, (bits + s.passes - 1) / s.passes);
   s.tiles = ceil_div64(n, SORT_TILE);
   return s;
+}
+int log_lanes(int64_t chunks, int most) {       // the smallest team that holds a row's chunks, at most 2^most lanes
+  int l = 0;
+  while (l < most && (1 << l) < chunks) ++l;
+  return l;
+}
+// Pairs per window: long windows leave fewer sums to join, short ones make more teams; the longest of 8 .. 64 that still gives the
+// chip 4096 waves (16 per CU) of 16-bit columns.
+int window_of(int64_t n, int64_t width) {
+  const int64_t chunks = ceil_div64(width, 8);
+  const int l = log_lanes(chunks, 8);
+  const int64_t lanes = ceil_div64(chunks, 1 << l) << l;
+  int w = 64;
+  while (w > 8 && (ceil_div64(n, w) * lanes < 4096 * 64 || (256 >> l) * w > SEG_PAIRS)) w >>= 1;
+  return w;
 }
 struct work_layout { int64_t a, b, counts, totals, heads, rank, part, bytes; };
 work_layout layout(int64_t n, int64_t width, int64_t num_rows) {
@@ -455,41 +593,45 @@ work_layout layout(int64_t n, int64_t width, int64_t num_rows) {
   l.totals = take(4LL << s.digit);
   l.heads = take(s.tiles * 4);
   l.rank = take(n * 4);
-  l.part = take(2 * ceil_div64(n, WINDOW) * width * 4);
+  l.part = take(2 * ceil_div64(n, window_of(n, width)) * width * 4);
   l.bytes = o;
   return l;
 }
-int log_lanes(int64_t chunks) {       // the smallest team that holds a row's chunks, at most a wave
-  int l = 0;
-  while (l < 6 && (1 << l) < chunks) ++l;
-  return l;
-}
-
-template <class TI, class TO>
-int launch_sums(seg_args a, hipStream_t stream) {
-  constexpr int VEC = elems16<TI>;
-  const bool wide = a.width >= VEC;
-  a.chunks = wide ? (a.width + VEC - 1) / VEC : a.width;
-  a.log_l = log_lanes(a.chunks);
-  const int64_t windows = ceil_div64(a.n, WINDOW);
-  dim3 grid((unsigned)ceil_div64(windows, 256 >> a.log_l), (unsigned)ceil_div64(a.chunks, 1 << a.log_l));
-  if (wide) k_segment_sum<TI, TO, VEC><<<grid, 256, 0, stream>>>(a);
-  else k_segment_sum<TI, TO, 1><<<grid, 256, 0, stream>>>(a);
+template <class TI, class TO, int VEC>
+int launch_sums_vec(seg_args a, bool accumulate, hipStream_t stream) {
+  a.chunks = VEC == 1 ? a.width : (a.width + VEC - 1) / VEC;
+  a.log_l = log_lanes(a.chunks, 8);
+  a.col_blocks = (int)ceil_div64(a.chunks, 1 << a.log_l);
+  const int64_t windows = ceil_div64(a.n, a.window), blocks = ceil_div64(windows, 256 >> a.log_l) * a.col_blocks;
+  ORCA_REQUIRE(blocks < (1LL << 31), "orca_embedding_backward: %lld ids of width %d are too many for one call", (long long)a.n, a.width);
+  if (accumulate) k_segment_sum<TI, TO, VEC, true><<<(unsigned)blocks, 256, 0, stream>>>(a);
+  else k_segment_sum<TI, TO, VEC, false><<<(unsigned)blocks, 256, 0, stream>>>(a);
   ORCA_LAUNCH_CHECK();
+  return ORCA_OK;
+}
+template <class TI, class TO>
+int launch_sums(seg_args a, bool accumulate, hipStream_t stream) {
+  constexpr int VEC = elems16<TI>;
+  if (int rc = a.width >= VEC ? launch_sums_vec<TI, TO, VEC>(a, accumulate, stream) : launch_sums_vec<TI, TO, 1>(a, accumulate, stream)) return rc;
+  const int64_t windows = ceil_div64(a.n, a.window);
   if (windows < 2) return ORCA_OK;
   a.chunks = (a.width + 3) / 4;
-  a.log_l = log_lanes(a.chunks);
-  k_segment_join<TO><<<dim3((unsigned)(windows - 1), (unsigned)ceil_div64(a.chunks, 1 << a.log_l)), 256, 0, stream>>>(a);
+  a.log_l = log_lanes(a.chunks, 6);
+  a.col_blocks = (int)ceil_div64(a.chunks, 1 << a.log_l);
+  const int64_t blocks = ceil_div64(windows - 1, 256 >> a.log_l) * a.col_blocks;
+  ORCA_REQUIRE(blocks < (1LL << 31), "orca_embedding_backward: %lld ids of width %d are too many for one call", (long long)a.n, a.width);
+  if (accumulate) k_segment_join<TO, true><<<(unsigned)blocks, 256, 0, stream>>>(a);
+  else k_segment_join<TO, false><<<(unsigned)blocks, 256, 0, stream>>>(a);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
 
-int sum_by_type(int g_dtype, int out_dtype, const seg_args& a, hipStream_t stream) {
+int sum_by_type(int g_dtype, int out_dtype, const seg_args& a, bool accumulate, hipStream_t stream) {
   if (out_dtype == ORCA_F32) {
-    if (g_dtype == ORCA_F32) return launch_sums<float, float>(a, stream);
-    return g_dtype == ORCA_BF16 ? launch_sums<__bf16, float>(a, stream) : launch_sums<_Float16, float>(a, stream);
+    if (g_dtype == ORCA_F32) return launch_sums<float, float>(a, accumulate, stream);
+    return g_dtype == ORCA_BF16 ? launch_sums<__bf16, float>(a, accumulate, stream) : launch_sums<_Float16, float>(a, accumulate, stream);
   }
-  return g_dtype == ORCA_BF16 ? launch_sums<__bf16, __bf16>(a, stream) : launch_sums<_Float16, _Float16>(a, stream);
+  return g_dtype == ORCA_BF16 ? launch_sums<__bf16, __bf16>(a, accumulate, stream) : launch_sums<_Float16, _Float16>(a, accumulate, stream);
 }
 
 int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, const int64_t* idx64, const int32_t* idx32, int64_t n, int64_t width,
@@ -507,20 +649,31 @@ int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, co
   return ORCA_OK;
 }
 
-// sorts (id, position); *sorted = where the result lies
+// the pieces of a fill that launch `i` of `launches` takes, and the workgroups for them
+unsigned fill_share(fill_job* f, int64_t pieces, int i, int launches) {
+  f->from = pieces * i / launches;
+  f->to = pieces * (i + 1) / launches;
+  return (unsigned)std::min<int64_t>(f->to - f->from, 4096);
+}
+
+// sorts (id, position), zeroes the fill's pieces on the way; *sorted = where the result lies
 int sort_positions(const int64_t* idx64, const int32_t* idx32, int64_t n, int64_t num_rows, int64_t padding, char* ws, const work_layout& l,
-                   const pair32** sorted, hipStream_t stream) {
+                   fill_job fill, int64_t pieces, const pair32** sorted, hipStream_t stream) {
   const sort_plan s = plan_sort(n, num_rows);
   sort_src src{idx64, idx32, nullptr, n, num_rows, padding};
   uint32_t* counts = (uint32_t*)(ws + l.counts);
-  uint32_t* totals = (uint32_t*)(ws + l.totals);
+  uint32_t* totals = s.tiles > DIRECT_TILES ? (uint32_t*)(ws + l.totals) : nullptr;
   pair32* buf[2] = {(pair32*)(ws + l.a), (pair32*)(ws + l.b)};
   for (int p = 0; p < s.passes; ++p) {
-    k_sort_count<<<(unsigned)s.tiles, SORT_THREADS, 0, stream>>>(src, p * s.digit, 1 << s.digit, counts);
+    unsigned extra = fill_share(&fill, pieces, 2 * p, 2 * s.passes);
+    k_sort_count<<<(unsigned)s.tiles + extra, SORT_THREADS, 0, stream>>>(src, p * s.digit, 1 << s.digit, counts, (int)s.tiles, fill);
     ORCA_LAUNCH_CHECK();
-    k_sort_columns<<<((1 << s.digit) + 63) / 64, 64, 0, stream>>>(counts, s.tiles, 1 << s.digit, totals);
-    ORCA_LAUNCH_CHECK();
-    k_sort_scatter<<<(unsigned)s.tiles, SORT_THREADS, 0, stream>>>(src, p * s.digit, s.digit, counts, totals, buf[p & 1]);
+    if (totals) {
+      k_sort_columns<<<((1 << s.digit) + 63) / 64, 64, 0, stream>>>(counts, s.tiles, 1 << s.digit, totals);
+      ORCA_LAUNCH_CHECK();
+    }
+    extra = fill_share(&fill, pieces, 2 * p + 1, 2 * s.passes);
+    k_sort_scatter<<<(unsigned)s.tiles + extra, SORT_THREADS, 0, stream>>>(src, p * s.digit, s.digit, counts, totals, buf[p & 1], (int)s.tiles, fill);
     ORCA_LAUNCH_CHECK();
     src.pairs = buf[p & 1];
   }
@@ -557,21 +710,29 @@ ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64
     return rc;
   if (num_rows == 0) return ORCA_OK;
   ORCA_REQUIRE(grad_table && (ld_table >= width || num_rows == 1), "orca_embedding_backward: null table, or rows that overlap");
+  fill_job fill{};
+  int64_t pieces = 0;
   if (!accumulate) {
     const int64_t e = table_dtype == ORCA_F32 ? 4 : 2;
     const bool gaps = ld_table != width && num_rows > 1;
-    const int64_t rows = gaps ? num_rows : 1, bytes = (gaps ? width : num_rows * width) * e;
-    k_zero_rows<<<(unsigned)std::min<int64_t>(2048, ceil_div64(rows * ceil_div64(bytes, 16), 256)), 256, 0, stream>>>((char*)grad_table, rows, bytes,
-                                                                                                                  ld_table * e);
-    ORCA_LAUNCH_CHECK();
+    fill.p = (char*)grad_table;
+    fill.bytes = (gaps ? width : num_rows * width) * e;
+    fill.pitch = ld_table * e;
+    fill.per_row = ceil_div64(fill.bytes, FILL_PIECE);
+    pieces = (gaps ? num_rows : 1) * fill.per_row;
   }
-  if (n == 0) return ORCA_OK;
+  if (n == 0) {
+    if (pieces) k_fill<<<fill_share(&fill, pieces, 0, 1), 512, 0, stream>>>(fill);
+    ORCA_LAUNCH_CHECK();
+    return ORCA_OK;
+  }
   const work_layout l = layout(n, width, num_rows);
   char* ws = (char*)workspace;
   const pair32* s = nullptr;
-  if (int rc = sort_positions(idx64, idx32, n, num_rows, padding_idx, ws, l, &s, stream)) return rc;
-  seg_args a{grad_out, ld_grad, n, ld_table, s, nullptr, grad_table, (float*)(ws + l.part), (int)width, 0, 0, accumulate != 0, (uint32_t)num_rows, scale};
-  return sum_by_type(grad_dtype, table_dtype, a, stream);
+  if (int rc = sort_positions(idx64, idx32, n, num_rows, padding_idx, ws, l, fill, pieces, &s, stream)) return rc;
+  seg_args a{grad_out, ld_grad, n, ld_table, s, nullptr, grad_table, (float*)(ws + l.part), (int)width, 0, 0, window_of(n, width), 0,
+             (uint32_t)num_rows, scale};
+  return sum_by_type(grad_dtype, table_dtype, a, accumulate != 0, stream);
 }
 
 ORCA_API int orca_embedding_backward_rows(const void* grad_out, int grad_dtype, int64_t ld_grad, const int64_t* idx64, const int32_t* idx32, int64_t n,
@@ -586,13 +747,13 @@ ORCA_API int orca_embedding_backward_rows(const void* grad_out, int grad_dtype, 
   const work_layout l = layout(n, width, num_rows);
   char* ws = (char*)workspace;
   const pair32* s = nullptr;
-  if (int rc = sort_positions(idx64, idx32, n, num_rows, padding_idx, ws, l, &s, stream)) return rc;
+  if (int rc = sort_positions(idx64, idx32, n, num_rows, padding_idx, ws, l, fill_job{}, 0, &s, stream)) return rc;
   const unsigned tiles = (unsigned)plan_sort(n, num_rows).tiles;
   uint32_t* rank = (uint32_t*)(ws + l.rank);
   k_rank_count<<<tiles, SORT_THREADS, 0, stream>>>(s, n, (uint32_t)num_rows, (uint32_t*)(ws + l.heads));
   ORCA_LAUNCH_CHECK();
   k_rank<<<tiles, SORT_THREADS, 0, stream>>>(s, n, (uint32_t)num_rows, (const uint32_t*)(ws + l.heads), rank, ids, count);
   ORCA_LAUNCH_CHECK();
-  seg_args a{grad_out, ld_grad, n, width, s, rank, rows, (float*)(ws + l.part), (int)width, 0, 0, 0, (uint32_t)num_rows, scale};
-  return sum_by_type(grad_dtype, rows_dtype, a, stream);
+  seg_args a{grad_out, ld_grad, n, width, s, rank, rows, (float*)(ws + l.part), (int)width, 0, 0, window_of(n, width), 0, (uint32_t)num_rows, scale};
+  return sum_by_type(grad_dtype, rows_dtype, a, false, stream);
 }
