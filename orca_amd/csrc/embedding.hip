@@ -195,14 +195,19 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v, int lane) {
   return v;
 }
 
-// the lanes of `in` whose digit equals this lane's
+// the lanes of `in` whose digit equals this lane's: per bit one compare, and one three-operand bit operation per half of the mask
 __device__ __forceinline__ uint64_t same_digit(uint32_t d, int digit_bits, bool in) {
-  uint64_t peers = __ballot(in);
-  for (int k = 0; k < digit_bits; ++k) {
-    const uint64_t m = __ballot((d >> k) & 1);
-    peers &= (d >> k) & 1 ? m : ~m;
+  const uint64_t all = __ballot(in);
+  uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
+#pragma unroll
+  for (int k = 0; k < MAX_DIGIT; ++k) {
+    if (k >= digit_bits) break;
+    const int bit = (int)(d << (31 - k)) >> 31;          // 0 or all ones
+    const uint64_t m = __ballot(bit != 0);
+    lo &= ~((uint32_t)m ^ (uint32_t)bit);
+    hi &= ~((uint32_t)(m >> 32) ^ (uint32_t)bit);
   }
-  return peers;
+  return ((uint64_t)hi << 32) | lo;
 }
 
 // totals == null: counts holds every tile's counts, which this workgroup adds up itself
@@ -271,13 +276,15 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
       const int b = 4 * t + k;
       place[b] = run + before[k];
       run += total[k];
-      uint32_t sum = 0;
+    }
+    uint64_t* four = reinterpret_cast<uint64_t*>(&part[0][0]) + t;      // four 16-bit counts, added up without a carry
+    uint64_t c[SORT_WAVES], sum = 0;
 #pragma unroll
-      for (int w = 0; w < SORT_WAVES; ++w) {
-        const uint32_t c = part[w][b];
-        part[w][b] = (uint16_t)sum;
-        sum += c;
-      }
+    for (int w = 0; w < SORT_WAVES; ++w) c[w] = four[w * (MAX_BINS / 4)];
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      four[w * (MAX_BINS / 4)] = sum;
+      sum += c[w];
     }
   }
   __syncthreads();
@@ -555,6 +562,240 @@ __global__ __launch_bounds__(256) void k_segment_join(seg_args a) {
   }
 }
 
+// ---- short lists: one launch -----------------------------------------------------------------------------------------
+// Up to SMALL_N ids (and SMALL_VALUES values) every workgroup sorts the whole list in its LDS -- some microseconds, the same in
+// all of them, against five launches that wait for one another -- and then takes its share of the distinct ids, of the column
+// blocks and of the table rows without an occurrence, which it zeroes (it knows them, so every row is written once).
+constexpr int SMALL_THREADS = 1024, SMALL_WAVES = 16, SMALL_ITEMS = 8, SMALL_N = SMALL_THREADS * SMALL_ITEMS;
+constexpr int64_t SMALL_VALUES = 1 << 20;      // beyond, a hub id's rows are too many for the one workgroup that adds them
+constexpr int SMALL_MAP = 65536;               // table rows of a workgroup's share, at most (bits in LDS)
+constexpr int SMALL_RUN = 32;                  // a longer run of equal ids is added by the whole workgroup ...
+constexpr int SMALL_TEAMS = 32;                // ... in at most this many consecutive parts
+struct small_args {
+  sort_src src;
+  const void* g;
+  int64_t ld_g, ld_out;
+  void* out;
+  int64_t* ids;                 // row-sparse form (or null): the distinct ids and their number
+  int32_t* count;
+  int n, width, chunks, log_l, col_blocks, passes, digit, zero_rows;
+  float scale;
+};
+struct small_lds { int part, heads, share, map, bytes; };          // byte offsets behind the pairs; what follows the sort lies over its counts
+__host__ __device__ inline small_lds small_layout(int n, int digit) {
+  const int items = (n + SMALL_THREADS - 1) / SMALL_THREADS;
+  small_lds l;
+  l.part = items * SMALL_THREADS * 8;
+  const int sort_end = l.part + (SMALL_WAVES * 2 << digit) + (4 << digit);
+  l.heads = l.part;
+  l.map = l.heads + (n + 2) / 2 * 4;
+  l.share = (l.map + SMALL_MAP / 8 + 15) / 16 * 16;
+  const int sums_end = l.share + SMALL_THREADS * 8 * 4;
+  l.bytes = sort_end > sums_end ? sort_end : sums_end;
+  return l;
+}
+
+template <class TI, class TO, int VEC, bool ACCUMULATE>
+__global__ __launch_bounds__(SMALL_THREADS) void k_small(small_args a) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ uint32_t wave_sum[SMALL_WAVES], queue[64];
+  __shared__ int queued;
+  const small_lds at = small_layout(a.n, a.digit);
+  pair32* list = (pair32*)lds;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = a.n, items = (n + SMALL_THREADS - 1) / SMALL_THREADS;
+  const int base = wave * 64 * items + lane, bins = 1 << a.digit;
+  const uint32_t none = (uint32_t)a.src.num_rows;
+  // the sort, as k_sort_scatter with one tile
+  uint16_t* part = (uint16_t*)(lds + at.part);                     // [wave][bin]
+  uint32_t* place = (uint32_t*)(lds + at.part + SMALL_WAVES * 2 * bins);
+  pair32 p[SMALL_ITEMS];
+#pragma unroll
+  for (int u = 0; u < SMALL_ITEMS; ++u) p[u] = u < items && base + 64 * u < n ? sort_read(a.src, base + 64 * u) : pair32{0u, 0u};
+  if (t == 0) queued = 0;
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const int shift = pass * a.digit;
+    for (int k = t; k < SMALL_WAVES * bins / 8; k += SMALL_THREADS) reinterpret_cast<u32x4*>(part)[k] = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    uint32_t rank[SMALL_ITEMS];
+#pragma unroll
+    for (int u = 0; u < SMALL_ITEMS; ++u) {
+      if (u >= items) break;
+      const bool in = base + 64 * u < n;
+      const uint32_t d = (p[u].key >> shift) & (uint32_t)(bins - 1);
+      const uint64_t peers = same_digit(d, a.digit, in);
+      const int leader = in ? __ffsll((unsigned long long)peers) - 1 : lane;
+      uint32_t seen = 0;
+      if (in && lane == leader) {
+        seen = part[wave * bins + d];
+        part[wave * bins + d] = (uint16_t)(seen + (uint32_t)__popcll(peers));
+      }
+      rank[u] = __shfl(seen, leader) + (uint32_t)__popcll(peers & ((1ULL << lane) - 1));
+    }
+    __syncthreads();
+    // a thread's two neighbouring bins lie in one word, and their counts (at most SMALL_N) add up without a carry
+    uint32_t total = 0;
+    if (2 * t < bins) {
+      uint32_t* two = reinterpret_cast<uint32_t*>(part) + t;
+      uint32_t c[SMALL_WAVES];
+#pragma unroll
+      for (int w = 0; w < SMALL_WAVES; ++w) c[w] = two[w * (bins >> 1)];
+#pragma unroll
+      for (int w = 0; w < SMALL_WAVES; ++w) {
+        two[w * (bins >> 1)] = total;
+        total += c[w];
+      }
+    }
+    const uint32_t mine = (total & 0xffff) + (total >> 16), inc = wave_inclusive(mine, lane);
+    if (lane == 63) wave_sum[wave] = inc;
+    __syncthreads();
+    uint32_t run = inc - mine;
+#pragma unroll
+    for (int w = 0; w < SMALL_WAVES; ++w) run += w < wave ? wave_sum[w] : 0u;
+    if (2 * t < bins) {
+      place[2 * t] = run;
+      place[2 * t + 1] = run + (total & 0xffff);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < SMALL_ITEMS; ++u) {
+      if (u >= items) break;
+      if (base + 64 * u < n) {
+        const uint32_t d = (p[u].key >> shift) & (uint32_t)(bins - 1);
+        list[place[d] + part[wave * bins + d] + rank[u]] = p[u];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < SMALL_ITEMS; ++u) {
+      if (u >= items) break;
+      if (base + 64 * u < n) p[u] = list[base + 64 * u];
+    }
+  }
+  // heads[r] = where the r-th distinct id's run begins; behind the last one, where the ids without a row begin
+  uint16_t* heads = (uint16_t*)(lds + at.heads);
+  uint64_t flags[SMALL_ITEMS];
+  uint32_t mine = 0;
+#pragma unroll
+  for (int u = 0; u < SMALL_ITEMS; ++u) {
+    if (u >= items) break;
+    const int i = base + 64 * u;
+    flags[u] = __ballot(i < n && p[u].key != none && (i == 0 || list[i - 1].key != p[u].key));
+    mine += (uint32_t)__popcll(flags[u]);
+  }
+  __syncthreads();                    // (wave_sum is read by the last pass, the counts by its scatter)
+  if (lane == 0) wave_sum[wave] = mine;
+  uint32_t* map = (uint32_t*)(lds + at.map);
+  const int64_t row0 = a.zero_rows ? a.src.num_rows * (int64_t)blockIdx.x / gridDim.x : 0;
+  const int rows = a.zero_rows ? (int)(a.src.num_rows * (int64_t)(blockIdx.x + 1) / gridDim.x - row0) : 0;
+  for (int k = t; k < (rows + 31) / 32; k += SMALL_THREADS) map[k] = 0;
+  __syncthreads();
+  uint32_t run = 0, distinct = 0;
+#pragma unroll
+  for (int w = 0; w < SMALL_WAVES; ++w) {
+    const uint32_t c = wave_sum[w];
+    run += w < wave ? c : 0u;
+    distinct += c;
+  }
+#pragma unroll
+  for (int u = 0; u < SMALL_ITEMS; ++u) {
+    if (u >= items) break;
+    const int i = base + 64 * u;
+    if ((flags[u] >> lane) & 1) {
+      heads[run + (uint32_t)__popcll(flags[u] & ((1ULL << lane) - 1))] = (uint16_t)i;
+      const int64_t r = (int64_t)p[u].key - row0;
+      if (r >= 0 && r < rows) atomicOr(&map[r >> 5], 1u << (r & 31));
+    }
+    run += (uint32_t)__popcll(flags[u]);
+    if (i < n && p[u].key == none && (i == 0 || list[i - 1].key != none)) heads[distinct] = (uint16_t)i;
+    if (i == n - 1 && p[u].key != none) heads[distinct] = (uint16_t)n;
+  }
+  __syncthreads();
+  if (a.count && blockIdx.x == 0 && t == 0) *a.count = (int32_t)distinct;
+  // zeros: a wave takes rows of its workgroup's share, or a lane does where a row is shorter than 16 bytes
+  if (rows > 0) {
+    const int bytes = a.width * (int)sizeof(TO), pieces = bytes < 16 ? 1 : (bytes + 15) / 16;
+    int lz = 0;
+    while (lz < 6 && (1 << lz) < pieces) ++lz;
+    for (int r = t >> lz; r < rows; r += SMALL_THREADS >> lz) {
+      if ((map[r >> 5] >> (r & 31)) & 1) continue;
+      TO* o = (TO*)a.out + (row0 + r) * a.ld_out;
+      if (bytes < 16) {
+        for (int j = 0; j < a.width; ++j) o[j] = (TO)0.f;
+      } else {
+        for (int k = t & ((1 << lz) - 1); k < pieces; k += 1 << lz) store16((char*)o + min(16 * k, bytes - 16), u32x4{0, 0, 0, 0});
+      }
+    }
+  }
+  // sums: this workgroup's distinct ids and columns
+  const int share = (int)gridDim.x / a.col_blocks, sh = (int)blockIdx.x / a.col_blocks;
+  const int r0 = (int)((int64_t)distinct * sh / share), r1 = (int)((int64_t)distinct * (sh + 1) / share);
+  const int teams = SMALL_THREADS >> a.log_l, team = t >> a.log_l, tl = t & ((1 << a.log_l) - 1);
+  const int c = ((int)blockIdx.x % a.col_blocks << a.log_l) + tl;
+  const int col = VEC == 1 ? c : min(c * VEC, a.width - VEC), own = c * VEC - col;
+  const bool live = c < a.chunks;
+  const TI* g = (const TI*)a.g + (live ? col : 0);
+  auto sum = [&](float (&acc)[VEC], int b, int e) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    for (int k = b; k < e; k += SEG_U) {
+      raw_chunk<VEC, TI> v[SEG_U];
+#pragma unroll
+      for (int u = 0; u < SEG_U; ++u) v[u].load(g + (int64_t)list[min(k + u, e - 1)].pos * a.ld_g);
+#pragma unroll
+      for (int u = 0; u < SEG_U; ++u)
+        if (k + u < e) v[u].add_to(acc);
+    }
+  };
+  auto write = [&](int r, const float (&acc)[VEC]) {
+    const uint32_t key = list[heads[r]].key;
+    if (a.ids && tl == 0 && c == tl) a.ids[r] = (int64_t)key;
+    TO* o = (TO*)a.out + (int64_t)(a.ids ? (uint32_t)r : key) * a.ld_out + col;
+    float f[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = acc[j] * a.scale;
+    if constexpr (ACCUMULATE) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (j >= own) o[j] = (TO)((float)o[j] + f[j]);
+    } else {
+      store_chunk<VEC, TO>(o, f);
+    }
+  };
+  float acc[VEC];
+  for (int q0 = r0; q0 < r1; q0 += 64) {          // 64 runs at a time: the queue's room
+    for (int r = q0 + team; r < min(r1, q0 + 64); r += teams) {
+      const int b = heads[r], e = heads[r + 1];
+      if (e - b > SMALL_RUN) {
+        if (tl == 0) queue[atomicAdd(&queued, 1)] = (uint32_t)r;
+      } else if (live) {
+        sum(acc, b, e);
+        write(r, acc);
+      }
+    }
+    __syncthreads();
+    const int todo = queued, most = min(teams, SMALL_TEAMS);
+    float* parts = (float*)(lds + at.share);
+    for (int q = 0; q < todo; ++q) {
+      const int r = (int)queue[q], b = heads[r], e = heads[r + 1], each = (e - b + most - 1) / most;
+      if (team < most && live) {
+        sum(acc, min(e, b + team * each), min(e, b + (team + 1) * each));
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) parts[t * VEC + j] = acc[j];
+      }
+      __syncthreads();
+      if (team == 0 && live) {
+        for (int k = 1; k < most; ++k)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] += parts[((k << a.log_l) + tl) * VEC + j];
+        write(r, acc);
+      }
+      __syncthreads();
+    }
+    if (t == 0) queued = 0;
+    __syncthreads();
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------
 struct sort_plan { int passes, digit; int64_t tiles; };
 sort_plan plan_sort(int64_t n, int64_t num_rows) {
@@ -632,6 +873,43 @@ int sum_by_type(int g_dtype, int out_dtype, const seg_args& a, bool accumulate, 
     return g_dtype == ORCA_BF16 ? launch_sums<__bf16, float>(a, accumulate, stream) : launch_sums<_Float16, float>(a, accumulate, stream);
   }
   return g_dtype == ORCA_BF16 ? launch_sums<__bf16, __bf16>(a, accumulate, stream) : launch_sums<_Float16, _Float16>(a, accumulate, stream);
+}
+
+bool is_small(int64_t n, int64_t width, int64_t num_rows) {
+  return n <= SMALL_N && n * width <= SMALL_VALUES && num_rows <= 256LL * SMALL_MAP;
+}
+template <class TI, class TO, int VEC, bool ACCUMULATE>
+int launch_small(small_args a, hipStream_t stream) {
+  static bool seen[64] = {};
+  if (orca_first_use_on_device(seen))
+    ORCA_HIP_TRY(hipFuncSetAttribute((const void*)k_small<TI, TO, VEC, ACCUMULATE>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                     small_layout(SMALL_N, MAX_DIGIT).bytes));
+  a.chunks = VEC == 1 ? a.width : (a.width + VEC - 1) / VEC;
+  a.log_l = log_lanes(a.chunks, 6);
+  a.col_blocks = (int)ceil_div64(a.chunks, 1 << a.log_l);
+  // workgroups: a distinct id per team, 128 KB of zeros or 65,536 rows each, at most one per CU (and one for each column block)
+  int64_t want = ceil_div64(a.n, SMALL_THREADS >> a.log_l) * a.col_blocks;
+  if (a.zero_rows) want = std::max({want, ceil_div64(a.src.num_rows * a.width * (int64_t)sizeof(TO), 131072), ceil_div64(a.src.num_rows, SMALL_MAP)});
+  const int64_t shares = std::max<int64_t>(1, ceil_div64(std::min<int64_t>(want, 256), a.col_blocks));
+  k_small<TI, TO, VEC, ACCUMULATE><<<(unsigned)(shares * a.col_blocks), SMALL_THREADS, small_layout(a.n, a.digit).bytes, stream>>>(a);
+  ORCA_LAUNCH_CHECK();
+  return ORCA_OK;
+}
+template <class TI, class TO>
+int small_typed(const small_args& a, bool accumulate, hipStream_t stream) {
+  constexpr int VEC = elems16<TI>;
+  if (a.width >= VEC) return accumulate ? launch_small<TI, TO, VEC, true>(a, stream) : launch_small<TI, TO, VEC, false>(a, stream);
+  return accumulate ? launch_small<TI, TO, 1, true>(a, stream) : launch_small<TI, TO, 1, false>(a, stream);
+}
+int small_by_type(int g_dtype, int out_dtype, small_args a, bool accumulate, hipStream_t stream) {
+  const sort_plan s = plan_sort(a.n, a.src.num_rows);
+  a.passes = s.passes;
+  a.digit = s.digit;
+  if (out_dtype == ORCA_F32) {
+    if (g_dtype == ORCA_F32) return small_typed<float, float>(a, accumulate, stream);
+    return g_dtype == ORCA_BF16 ? small_typed<__bf16, float>(a, accumulate, stream) : small_typed<_Float16, float>(a, accumulate, stream);
+  }
+  return g_dtype == ORCA_BF16 ? small_typed<__bf16, __bf16>(a, accumulate, stream) : small_typed<_Float16, _Float16>(a, accumulate, stream);
 }
 
 int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, const int64_t* idx64, const int32_t* idx32, int64_t n, int64_t width,
@@ -726,6 +1004,12 @@ ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64
     ORCA_LAUNCH_CHECK();
     return ORCA_OK;
   }
+  if (is_small(n, width, num_rows)) {
+    small_args a{{idx64, idx32, nullptr, n, num_rows, padding_idx}, grad_out, ld_grad, ld_table, grad_table, nullptr, nullptr, (int)n, (int)width};
+    a.zero_rows = !accumulate;
+    a.scale = scale;
+    return small_by_type(grad_dtype, table_dtype, a, accumulate != 0, stream);
+  }
   const work_layout l = layout(n, width, num_rows);
   char* ws = (char*)workspace;
   const pair32* s = nullptr;
@@ -744,6 +1028,11 @@ ORCA_API int orca_embedding_backward_rows(const void* grad_out, int grad_dtype, 
     return rc;
   ORCA_REQUIRE(count && (n == 0 || (ids && rows)), "orca_embedding_backward_rows: null output");
   if (n == 0) return orca_fill_i32(count, 1, 0, stream_);
+  if (is_small(n, width, num_rows)) {
+    small_args a{{idx64, idx32, nullptr, n, num_rows, padding_idx}, grad_out, ld_grad, width, rows, ids, count, (int)n, (int)width};
+    a.scale = scale;
+    return small_by_type(grad_dtype, rows_dtype, a, false, stream);
+  }
   const work_layout l = layout(n, width, num_rows);
   char* ws = (char*)workspace;
   const pair32* s = nullptr;
