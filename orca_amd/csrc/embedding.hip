@@ -562,67 +562,132 @@ __global__ __launch_bounds__(256) void k_segment_join(seg_args a) {
   }
 }
 
-// ---- short lists: one launch -----------------------------------------------------------------------------------------
-// Up to SMALL_N ids (and SMALL_VALUES values) every workgroup sorts the whole list in its LDS -- some microseconds, the same in
-// all of them, against five launches that wait for one another -- and then takes its share of the distinct ids, of the column
-// blocks and of the table rows without an occurrence, which it zeroes (it knows them, so every row is written once).
-constexpr int SMALL_THREADS = 1024, SMALL_WAVES = 16, SMALL_ITEMS = 8, SMALL_N = SMALL_THREADS * SMALL_ITEMS;
+// ---- short lists -----------------------------------------------------------------------------------------------------
+// Up to SMALL_N ids (and SMALL_VALUES values) there is no order of the whole list to build: every workgroup reads all the ids (26 KB
+// for 6600 of them, out of L2), keeps its share in the order of their positions and sorts those few in LDS.
+//   dense, one launch (k_small): a hash of the id gives it to a workgroup, which adds its ids' rows.  It also has a share of the
+//          table's rows; it marks those with an occurrence and zeroes the others, so that every row is written once.
+//   rows, two launches: k_range_sort gives a workgroup the ids of an equal share of [0, num_rows), so that its sorted ids follow
+//          those of the workgroup before; it leaves their positions and the number of distinct ones.  k_range_sums adds those numbers
+//          up, which tells where every distinct id's row lies, and takes an even share of the runs.
+// Against it: the general path's launches wait for one another (600 ids 28 us, 6600 row-sparse 38 us); the whole list sorted by
+// every workgroup took 9 us per radix pass at 6600 ids; the rows' places counted within one launch, over a hash set of all ids,
+// took 24 us.
+constexpr int SMALL_THREADS = 1024, SMALL_ITEMS = 8, SMALL_N = SMALL_THREADS * SMALL_ITEMS;
+constexpr int TINY_THREADS = 256, TINY_N = TINY_THREADS * SMALL_ITEMS;         // workgroups of four waves: cheaper barriers
 constexpr int64_t SMALL_VALUES = 1 << 20;      // beyond, a hub id's rows are too many for the one workgroup that adds them
 constexpr int SMALL_MAP = 65536;               // table rows of a workgroup's share, at most (bits in LDS)
 constexpr int SMALL_RUN = 32;                  // a longer run of equal ids is added by the whole workgroup ...
 constexpr int SMALL_TEAMS = 32;                // ... in at most this many consecutive parts
+constexpr int SMALL_PAIRS = 128;               // up to this many pairs are sorted by counting the smaller ones, one thread per pair
+constexpr int SMALL_DIGIT = 8;                 // digit bits of the sort of longer lists
+constexpr int MAX_RANGES = 256;
 struct small_args {
-  sort_src src;
+  const int64_t* idx64;
+  const int32_t* idx32;
+  int64_t num_rows, padding;
   const void* g;
   int64_t ld_g, ld_out;
   void* out;
-  int64_t* ids;                 // row-sparse form (or null): the distinct ids and their number
-  int32_t* count;
-  int n, width, chunks, log_l, col_blocks, passes, digit, zero_rows;
+  int n, width, chunks, log_l, col_blocks, zero_rows;
   float scale;
 };
-struct small_lds { int part, heads, share, map, bytes; };          // byte offsets behind the pairs; what follows the sort lies over its counts
-__host__ __device__ inline small_lds small_layout(int n, int digit) {
-  const int items = (n + SMALL_THREADS - 1) / SMALL_THREADS;
+// LDS: the list (room for all n: they may be equal, or meet in one hash), and one region in turn for the bit map, the sort's counts,
+// and the sums: the parts of a long run and the starts of the runs
+struct small_lds { int region, heads, bytes; };
+__host__ __device__ inline small_lds small_layout(int threads, int n) {
   small_lds l;
-  l.part = items * SMALL_THREADS * 8;
-  const int sort_end = l.part + (SMALL_WAVES * 2 << digit) + (4 << digit);
-  l.heads = l.part;
-  l.map = l.heads + (n + 2) / 2 * 4;
-  l.share = (l.map + SMALL_MAP / 8 + 15) / 16 * 16;
-  const int sums_end = l.share + SMALL_THREADS * 8 * 4;
-  l.bytes = sort_end > sums_end ? sort_end : sums_end;
+  l.region = (n + (n & 1)) * 8;
+  l.heads = l.region + threads * 8 * 4;
+  l.bytes = l.heads + 2 * (n + 1);
   return l;
 }
+static_assert(((TINY_THREADS / 64 * 2 + 4) << SMALL_DIGIT) <= TINY_THREADS * 32 && ((SMALL_THREADS / 64 * 2 + 4) << SMALL_DIGIT) <= SMALL_THREADS * 32 &&
+                  SMALL_MAP / 8 <= TINY_THREADS * 32,
+              "the sort's counts and the bit map fit where the parts of a run lie");
+// MurmurHash3's finaliser: ids in arithmetic progression (a multiplicative hash keeps them in one) land all over the range
+__device__ __forceinline__ uint32_t small_hash(uint32_t key) {
+  key ^= key >> 16;
+  key *= 0x85ebca6bu;
+  key ^= key >> 13;
+  key *= 0xc2b2ae35u;
+  return key ^ key >> 16;
+}
 
-template <class TI, class TO, int VEC, bool ACCUMULATE>
-__global__ __launch_bounds__(SMALL_THREADS) void k_small(small_args a) {
-  extern __shared__ __align__(16) char lds[];
-  __shared__ uint32_t wave_sum[SMALL_WAVES], queue[64];
-  __shared__ int queued;
-  const small_lds at = small_layout(a.n, a.digit);
-  pair32* list = (pair32*)lds;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = a.n, items = (n + SMALL_THREADS - 1) / SMALL_THREADS;
-  const int base = wave * 64 * items + lane, bins = 1 << a.digit;
-  const uint32_t none = (uint32_t)a.src.num_rows;
-  // the sort, as k_sort_scatter with one tile
-  uint16_t* part = (uint16_t*)(lds + at.part);                     // [wave][bin]
-  uint32_t* place = (uint32_t*)(lds + at.part + SMALL_WAVES * 2 * bins);
+// this thread's ids: pair i = base + 64 * u, `none` for what has no row
+template <int THREADS>
+__device__ __forceinline__ void small_keys(const small_args& a, int base, int items, uint32_t (&key)[SMALL_ITEMS]) {
+#pragma unroll
+  for (int u = 0; u < SMALL_ITEMS; ++u) {
+    key[u] = (uint32_t)a.num_rows;
+    if (u < items && base + 64 * u < a.n) {
+      const int64_t id = a.idx64 ? a.idx64[base + 64 * u] : (int64_t)a.idx32[base + 64 * u];
+      if (id >= 0 && id < a.num_rows && id != a.padding) key[u] = (uint32_t)id;
+    }
+  }
+}
+// numbers 0, 1, .. for the set flags of a wave-by-wave list; returns this wave's first number, *all = how many there are.  Two barriers.
+template <int THREADS>
+__device__ __forceinline__ uint32_t small_offsets(uint32_t mine, uint32_t* wave_sum, uint32_t* all) {
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) wave_sum[wave] = mine;
+  __syncthreads();
+  uint32_t run = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const uint32_t c = wave_sum[w];
+    run += w < wave ? c : 0u;
+    sum += c;
+  }
+  __syncthreads();
+  *all = sum;
+  return run;
+}
+
+// sorts the first `m` pairs of `list` by key - least < 2^bits, equal keys in the order they had; all threads of the workgroup call it
+template <int THREADS>
+__device__ __forceinline__ void small_sort(pair32* list, int m, uint32_t least, int bits, char* region, uint32_t* wave_sum) {
+  constexpr int WAVES = THREADS / 64;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  if (m <= SMALL_PAIRS) {
+    static_assert(SMALL_PAIRS == 128, "two waves of pairs");
+    pair32 p{0u, ~0u};
+    int rank = 0;
+    if (wave < 2) {
+      const uint32_t lo = lane < m ? list[lane].key : ~0u, hi = 64 + lane < m ? list[64 + lane].key : ~0u;
+      if (t < m) p = pair32{list[t].pos, wave ? hi : lo};
+      for (int j = 0; j < min(m, 64); ++j) {
+        const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)lo, j);
+        rank += key < p.key || (key == p.key && j < t);
+      }
+      for (int j = 64; j < m; ++j) {
+        const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)hi, j - 64);
+        rank += key < p.key || (key == p.key && j < t);
+      }
+    }
+    __syncthreads();
+    if (t < m) list[rank] = p;
+    __syncthreads();
+    return;
+  }
+  const int items = (m + THREADS - 1) / THREADS, base = wave * 64 * items + lane;
+  const int passes = (bits + SMALL_DIGIT - 1) / SMALL_DIGIT, digit = max(MIN_DIGIT, (bits + passes - 1) / passes), bins = 1 << digit;
+  uint16_t* part = (uint16_t*)region;                    // [wave][bin], as in k_sort_scatter
+  uint32_t* place = (uint32_t*)(region + WAVES * 2 * bins);
   pair32 p[SMALL_ITEMS];
 #pragma unroll
-  for (int u = 0; u < SMALL_ITEMS; ++u) p[u] = u < items && base + 64 * u < n ? sort_read(a.src, base + 64 * u) : pair32{0u, 0u};
-  if (t == 0) queued = 0;
-  for (int pass = 0; pass < a.passes; ++pass) {
-    const int shift = pass * a.digit;
-    for (int k = t; k < SMALL_WAVES * bins / 8; k += SMALL_THREADS) reinterpret_cast<u32x4*>(part)[k] = u32x4{0, 0, 0, 0};
+  for (int u = 0; u < SMALL_ITEMS; ++u) p[u] = u < items && base + 64 * u < m ? list[base + 64 * u] : pair32{0u, least};
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * digit;
+    for (int k = t; k < WAVES * bins / 8; k += THREADS) reinterpret_cast<u32x4*>(part)[k] = u32x4{0, 0, 0, 0};
     __syncthreads();
     uint32_t rank[SMALL_ITEMS];
 #pragma unroll
     for (int u = 0; u < SMALL_ITEMS; ++u) {
       if (u >= items) break;
-      const bool in = base + 64 * u < n;
-      const uint32_t d = (p[u].key >> shift) & (uint32_t)(bins - 1);
-      const uint64_t peers = same_digit(d, a.digit, in);
+      const bool in = base + 64 * u < m;
+      const uint32_t d = ((p[u].key - least) >> shift) & (uint32_t)(bins - 1);
+      const uint64_t peers = same_digit(d, digit, in);
       const int leader = in ? __ffsll((unsigned long long)peers) - 1 : lane;
       uint32_t seen = 0;
       if (in && lane == leader) {
@@ -636,21 +701,18 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_small(small_args a) {
     uint32_t total = 0;
     if (2 * t < bins) {
       uint32_t* two = reinterpret_cast<uint32_t*>(part) + t;
-      uint32_t c[SMALL_WAVES];
+      uint32_t c[WAVES];
 #pragma unroll
-      for (int w = 0; w < SMALL_WAVES; ++w) c[w] = two[w * (bins >> 1)];
+      for (int w = 0; w < WAVES; ++w) c[w] = two[w * (bins >> 1)];
 #pragma unroll
-      for (int w = 0; w < SMALL_WAVES; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         two[w * (bins >> 1)] = total;
         total += c[w];
       }
     }
     const uint32_t mine = (total & 0xffff) + (total >> 16), inc = wave_inclusive(mine, lane);
-    if (lane == 63) wave_sum[wave] = inc;
-    __syncthreads();
-    uint32_t run = inc - mine;
-#pragma unroll
-    for (int w = 0; w < SMALL_WAVES; ++w) run += w < wave ? wave_sum[w] : 0u;
+    uint32_t all;
+    const uint32_t run = small_offsets<THREADS>((uint32_t)__builtin_amdgcn_readlane((int)inc, 63), wave_sum, &all) + inc - mine;
     if (2 * t < bins) {
       place[2 * t] = run;
       place[2 * t + 1] = run + (total & 0xffff);
@@ -659,8 +721,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_small(small_args a) {
 #pragma unroll
     for (int u = 0; u < SMALL_ITEMS; ++u) {
       if (u >= items) break;
-      if (base + 64 * u < n) {
-        const uint32_t d = (p[u].key >> shift) & (uint32_t)(bins - 1);
+      if (base + 64 * u < m) {
+        const uint32_t d = ((p[u].key - least) >> shift) & (uint32_t)(bins - 1);
         list[place[d] + part[wave * bins + d] + rank[u]] = p[u];
       }
     }
@@ -668,69 +730,43 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_small(small_args a) {
 #pragma unroll
     for (int u = 0; u < SMALL_ITEMS; ++u) {
       if (u >= items) break;
-      if (base + 64 * u < n) p[u] = list[base + 64 * u];
+      if (base + 64 * u < m) p[u] = list[base + 64 * u];
     }
   }
-  // heads[r] = where the r-th distinct id's run begins; behind the last one, where the ids without a row begin
-  uint16_t* heads = (uint16_t*)(lds + at.heads);
-  uint64_t flags[SMALL_ITEMS];
-  uint32_t mine = 0;
+}
+
+// heads[r] = where the r-th run of equal keys begins, heads[distinct] = m; returns distinct
+template <int THREADS>
+__device__ __forceinline__ uint32_t small_heads(const pair32* list, int m, uint16_t* heads, uint32_t* wave_sum) {
+  const int lane = threadIdx.x & 63, items = (m + THREADS - 1) / THREADS, base = (threadIdx.x >> 6) * 64 * items + lane;
+  uint64_t take[SMALL_ITEMS];
+  uint32_t mine = 0, distinct;
 #pragma unroll
   for (int u = 0; u < SMALL_ITEMS; ++u) {
     if (u >= items) break;
     const int i = base + 64 * u;
-    flags[u] = __ballot(i < n && p[u].key != none && (i == 0 || list[i - 1].key != p[u].key));
-    mine += (uint32_t)__popcll(flags[u]);
+    take[u] = __ballot(i < m && (i == 0 || list[i - 1].key != list[i].key));
+    mine += (uint32_t)__popcll(take[u]);
   }
-  __syncthreads();                    // (wave_sum is read by the last pass, the counts by its scatter)
-  if (lane == 0) wave_sum[wave] = mine;
-  uint32_t* map = (uint32_t*)(lds + at.map);
-  const int64_t row0 = a.zero_rows ? a.src.num_rows * (int64_t)blockIdx.x / gridDim.x : 0;
-  const int rows = a.zero_rows ? (int)(a.src.num_rows * (int64_t)(blockIdx.x + 1) / gridDim.x - row0) : 0;
-  for (int k = t; k < (rows + 31) / 32; k += SMALL_THREADS) map[k] = 0;
-  __syncthreads();
-  uint32_t run = 0, distinct = 0;
-#pragma unroll
-  for (int w = 0; w < SMALL_WAVES; ++w) {
-    const uint32_t c = wave_sum[w];
-    run += w < wave ? c : 0u;
-    distinct += c;
-  }
+  uint32_t run = small_offsets<THREADS>(mine, wave_sum, &distinct);
 #pragma unroll
   for (int u = 0; u < SMALL_ITEMS; ++u) {
     if (u >= items) break;
-    const int i = base + 64 * u;
-    if ((flags[u] >> lane) & 1) {
-      heads[run + (uint32_t)__popcll(flags[u] & ((1ULL << lane) - 1))] = (uint16_t)i;
-      const int64_t r = (int64_t)p[u].key - row0;
-      if (r >= 0 && r < rows) atomicOr(&map[r >> 5], 1u << (r & 31));
-    }
-    run += (uint32_t)__popcll(flags[u]);
-    if (i < n && p[u].key == none && (i == 0 || list[i - 1].key != none)) heads[distinct] = (uint16_t)i;
-    if (i == n - 1 && p[u].key != none) heads[distinct] = (uint16_t)n;
+    if ((take[u] >> lane) & 1) heads[run + (uint32_t)__popcll(take[u] & ((1ULL << lane) - 1))] = (uint16_t)(base + 64 * u);
+    run += (uint32_t)__popcll(take[u]);
   }
+  if (threadIdx.x == 0) heads[distinct] = (uint16_t)m;
   __syncthreads();
-  if (a.count && blockIdx.x == 0 && t == 0) *a.count = (int32_t)distinct;
-  // zeros: a wave takes rows of its workgroup's share, or a lane does where a row is shorter than 16 bytes
-  if (rows > 0) {
-    const int bytes = a.width * (int)sizeof(TO), pieces = bytes < 16 ? 1 : (bytes + 15) / 16;
-    int lz = 0;
-    while (lz < 6 && (1 << lz) < pieces) ++lz;
-    for (int r = t >> lz; r < rows; r += SMALL_THREADS >> lz) {
-      if ((map[r >> 5] >> (r & 31)) & 1) continue;
-      TO* o = (TO*)a.out + (row0 + r) * a.ld_out;
-      if (bytes < 16) {
-        for (int j = 0; j < a.width; ++j) o[j] = (TO)0.f;
-      } else {
-        for (int k = t & ((1 << lz) - 1); k < pieces; k += 1 << lz) store16((char*)o + min(16 * k, bytes - 16), u32x4{0, 0, 0, 0});
-      }
-    }
-  }
-  // sums: this workgroup's distinct ids and columns
-  const int share = (int)gridDim.x / a.col_blocks, sh = (int)blockIdx.x / a.col_blocks;
-  const int r0 = (int)((int64_t)distinct * sh / share), r1 = (int)((int64_t)distinct * (sh + 1) / share);
-  const int teams = SMALL_THREADS >> a.log_l, team = t >> a.log_l, tl = t & ((1 << a.log_l) - 1);
-  const int c = ((int)blockIdx.x % a.col_blocks << a.log_l) + tl;
+  return distinct;
+}
+
+// Adds the rows of `runs` runs and hands each sum to put(run, acc, col, own).  begin(r), end(r): the run's pairs; pos(k): the position of
+// pair k.  A team of 2^log_l lanes takes a run; what is longer than SMALL_RUN waits for the whole workgroup, whose teams take a
+// consecutive part each.  All threads call it.
+template <int THREADS, class TI, int VEC, class B, class E, class P, class W>
+__device__ __forceinline__ void small_sums(const small_args& a, int runs, B begin, E end, P pos, W put, float* parts, uint32_t* queue, int* queued) {
+  const int t = threadIdx.x, teams = THREADS >> a.log_l, team = t >> a.log_l, tl = t & ((1 << a.log_l) - 1);
+  const int c = ((int)(blockIdx.x % (uint32_t)a.col_blocks) << a.log_l) + tl;
   const int col = VEC == 1 ? c : min(c * VEC, a.width - VEC), own = c * VEC - col;
   const bool live = c < a.chunks;
   const TI* g = (const TI*)a.g + (live ? col : 0);
@@ -740,43 +776,27 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_small(small_args a) {
     for (int k = b; k < e; k += SEG_U) {
       raw_chunk<VEC, TI> v[SEG_U];
 #pragma unroll
-      for (int u = 0; u < SEG_U; ++u) v[u].load(g + (int64_t)list[min(k + u, e - 1)].pos * a.ld_g);
+      for (int u = 0; u < SEG_U; ++u) v[u].load(g + (int64_t)pos(min(k + u, e - 1)) * a.ld_g);
 #pragma unroll
       for (int u = 0; u < SEG_U; ++u)
         if (k + u < e) v[u].add_to(acc);
     }
   };
-  auto write = [&](int r, const float (&acc)[VEC]) {
-    const uint32_t key = list[heads[r]].key;
-    if (a.ids && tl == 0 && c == tl) a.ids[r] = (int64_t)key;
-    TO* o = (TO*)a.out + (int64_t)(a.ids ? (uint32_t)r : key) * a.ld_out + col;
-    float f[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = acc[j] * a.scale;
-    if constexpr (ACCUMULATE) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (j >= own) o[j] = (TO)((float)o[j] + f[j]);
-    } else {
-      store_chunk<VEC, TO>(o, f);
-    }
-  };
   float acc[VEC];
-  for (int q0 = r0; q0 < r1; q0 += 64) {          // 64 runs at a time: the queue's room
-    for (int r = q0 + team; r < min(r1, q0 + 64); r += teams) {
-      const int b = heads[r], e = heads[r + 1];
+  for (int q0 = 0; q0 < runs; q0 += 64) {          // 64 runs at a time: the queue's room
+    for (int r = q0 + team; r < min(runs, q0 + 64); r += teams) {
+      const int b = begin(r), e = end(r);
       if (e - b > SMALL_RUN) {
-        if (tl == 0) queue[atomicAdd(&queued, 1)] = (uint32_t)r;
+        if (tl == 0) queue[atomicAdd(queued, 1)] = (uint32_t)r;
       } else if (live) {
         sum(acc, b, e);
-        write(r, acc);
+        put(r, acc, col, own);
       }
     }
     __syncthreads();
-    const int todo = queued, most = min(teams, SMALL_TEAMS);
-    float* parts = (float*)(lds + at.share);
+    const int todo = *queued, most = min(teams, SMALL_TEAMS);
     for (int q = 0; q < todo; ++q) {
-      const int r = (int)queue[q], b = heads[r], e = heads[r + 1], each = (e - b + most - 1) / most;
+      const int r = (int)queue[q], b = begin(r), e = end(r), each = (e - b + most - 1) / most;
       if (team < most && live) {
         sum(acc, min(e, b + team * each), min(e, b + (team + 1) * each));
 #pragma unroll
@@ -787,13 +807,193 @@ __global__ __launch_bounds__(SMALL_THREADS) void k_small(small_args a) {
         for (int k = 1; k < most; ++k)
 #pragma unroll
           for (int j = 0; j < VEC; ++j) acc[j] += parts[((k << a.log_l) + tl) * VEC + j];
-        write(r, acc);
+        put(r, acc, col, own);
       }
       __syncthreads();
     }
-    if (t == 0) queued = 0;
+    if (q0 + 64 < runs) {
+      if (t == 0) *queued = 0;
+      __syncthreads();
+    }
+  }
+}
+
+template <int THREADS, class TI, class TO, int VEC, bool ACCUMULATE>
+__global__ __launch_bounds__(THREADS) void k_small(small_args a, int bits) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ uint32_t wave_sum[THREADS / 64], queue[64];
+  __shared__ int queued;
+  const small_lds at = small_layout(THREADS, a.n);
+  pair32* list = (pair32*)lds;
+  uint16_t* heads = (uint16_t*)(lds + at.heads);
+  char* region = lds + at.region;
+  const int t = threadIdx.x, lane = t & 63, items = (a.n + THREADS - 1) / THREADS, base = (t >> 6) * 64 * items + lane;
+  const uint32_t none = (uint32_t)a.num_rows, share = gridDim.x / (uint32_t)a.col_blocks, sh = blockIdx.x / (uint32_t)a.col_blocks;
+  uint32_t key[SMALL_ITEMS];
+  small_keys<THREADS>(a, base, items, key);
+  // this workgroup's rows of the table, for the zeros
+  const int64_t row0 = a.zero_rows ? a.num_rows * (int64_t)blockIdx.x / gridDim.x : 0;
+  const int zeros = a.zero_rows ? (int)(a.num_rows * (int64_t)(blockIdx.x + 1) / gridDim.x - row0) : 0;
+  uint32_t* map = (uint32_t*)region;
+  for (int k = t; k < (zeros + 31) / 32; k += THREADS) map[k] = 0;
+  if (t == 0) queued = 0;
+  // the pairs that a hash gives this workgroup, in the order of their positions
+  uint64_t take[SMALL_ITEMS];
+  uint32_t mine = 0, m;
+#pragma unroll
+  for (int u = 0; u < SMALL_ITEMS; ++u) {
+    if (u >= items) break;
+    take[u] = __ballot(key[u] != none && __umulhi(small_hash(key[u]), share) == sh);
+    mine += (uint32_t)__popcll(take[u]);
+  }
+  uint32_t run = small_offsets<THREADS>(mine, wave_sum, &m);
+#pragma unroll
+  for (int u = 0; u < SMALL_ITEMS; ++u) {
+    if (u >= items) break;
+    if ((take[u] >> lane) & 1) list[run + (uint32_t)__popcll(take[u] & ((1ULL << lane) - 1))] = pair32{(uint32_t)(base + 64 * u), key[u]};
+    run += (uint32_t)__popcll(take[u]);
+    const int64_t r = (int64_t)key[u] - row0;
+    if (key[u] != none && r >= 0 && r < zeros) atomicOr(&map[r >> 5], 1u << (r & 31));
+  }
+  __syncthreads();
+  // zeros: a team of lanes takes a row, or a lane does where a row is shorter than 16 bytes
+  if (zeros > 0) {
+    const int bytes = a.width * (int)sizeof(TO), pieces = bytes < 16 ? 1 : (bytes + 15) / 16;
+    int lz = 0;
+    while (lz < 6 && (1 << lz) < pieces) ++lz;
+    for (int r = t >> lz; r < zeros; r += THREADS >> lz) {
+      if ((map[r >> 5] >> (r & 31)) & 1) continue;
+      TO* o = (TO*)a.out + (row0 + r) * a.ld_out;
+      if (bytes < 16) {
+        for (int j = 0; j < a.width; ++j) o[j] = (TO)0.f;
+      } else {
+        for (int k = t & ((1 << lz) - 1); k < pieces; k += 1 << lz) store16((char*)o + min(16 * k, bytes - 16), u32x4{0, 0, 0, 0});
+      }
+    }
     __syncthreads();
   }
+  small_sort<THREADS>(list, (int)m, 0u, bits, region, wave_sum);
+  const int distinct = (int)small_heads<THREADS>(list, (int)m, heads, wave_sum);
+  small_sums<THREADS, TI, VEC>(
+      a, distinct, [&](int r) { return (int)heads[r]; }, [&](int r) { return (int)heads[r + 1]; }, [&](int k) { return list[k].pos; },
+      [&](int r, const float (&acc)[VEC], int col, int own) {
+        TO* o = (TO*)a.out + (int64_t)list[heads[r]].key * a.ld_out + col;
+        float f[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] = acc[j] * a.scale;
+        if constexpr (ACCUMULATE) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (j >= own) o[j] = (TO)((float)o[j] + f[j]);
+        } else {
+          store_chunk<VEC, TO>(o, f);
+        }
+      },
+      (float*)region, queue, &queued);
+}
+
+// what k_range_sort leaves for k_range_sums
+struct range_work {
+  uint16_t* pos;                // [n] positions in the order of (id, position)
+  uint16_t* heads;              // [n] per range, at its first pair's place: where its runs begin, from there
+  uint32_t* key;                // [n] the runs' ids, beside heads
+  uint32_t* first;              // [ranges + 1] a range's first pair; how many there are
+  uint32_t* distinct;           // [ranges]
+};
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void k_range_sort(small_args a, range_work w) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ uint32_t wave_sum[THREADS / 64];
+  const small_lds at = small_layout(THREADS, a.n);
+  pair32* list = (pair32*)lds;
+  uint16_t* heads = (uint16_t*)(lds + at.heads);
+  const int t = threadIdx.x, lane = t & 63, items = (a.n + THREADS - 1) / THREADS, base = (t >> 6) * 64 * items + lane;
+  uint32_t key[SMALL_ITEMS];
+  small_keys<THREADS>(a, base, items, key);
+  const uint32_t lo = (uint32_t)(a.num_rows * (int64_t)blockIdx.x / gridDim.x), hi = (uint32_t)(a.num_rows * (int64_t)(blockIdx.x + 1) / gridDim.x);
+  uint64_t take[SMALL_ITEMS];
+  uint32_t mine = 0, below = 0, m, before;
+#pragma unroll
+  for (int u = 0; u < SMALL_ITEMS; ++u) {
+    if (u >= items) break;
+    take[u] = __ballot(key[u] >= lo && key[u] < hi);
+    mine += (uint32_t)__popcll(take[u]);
+    below += (uint32_t)__popcll(__ballot(key[u] < lo));
+  }
+  uint32_t run = small_offsets<THREADS>(mine, wave_sum, &m);
+  small_offsets<THREADS>(below, wave_sum, &before);
+#pragma unroll
+  for (int u = 0; u < SMALL_ITEMS; ++u) {
+    if (u >= items) break;
+    if ((take[u] >> lane) & 1) list[run + (uint32_t)__popcll(take[u] & ((1ULL << lane) - 1))] = pair32{(uint32_t)(base + 64 * u), key[u]};
+    run += (uint32_t)__popcll(take[u]);
+  }
+  __syncthreads();
+  int bits = 1;
+  while (((hi - lo) >> bits) != 0) ++bits;
+  small_sort<THREADS>(list, (int)m, lo, bits, lds + at.region, wave_sum);
+  const uint32_t distinct = small_heads<THREADS>(list, (int)m, heads, wave_sum);
+  for (int i = t; i < (int)m; i += THREADS) w.pos[before + i] = (uint16_t)list[i].pos;
+  for (int r = t; r < (int)distinct; r += THREADS) {
+    w.heads[before + r] = heads[r];
+    w.key[before + r] = list[heads[r]].key;
+  }
+  if (t == 0) {
+    w.first[blockIdx.x] = before;
+    w.distinct[blockIdx.x] = distinct;
+    if (blockIdx.x == gridDim.x - 1) w.first[gridDim.x] = before + m;
+  }
+}
+
+template <class TI, class TO, int VEC>
+__global__ __launch_bounds__(TINY_THREADS) void k_range_sums(small_args a, range_work w, int ranges, int64_t* __restrict__ ids, int32_t* __restrict__ count) {
+  __shared__ uint32_t wave_sum[TINY_THREADS / 64], queue[64], row[MAX_RANGES + 1], first[MAX_RANGES + 1];
+  __shared__ int queued;
+  __shared__ float parts[TINY_THREADS * 8];
+  static_assert(MAX_RANGES == TINY_THREADS, "a thread per range");
+  const int t = threadIdx.x, lane = t & 63;
+  const uint32_t mine = t < ranges ? w.distinct[t] : 0u, inc = wave_inclusive(mine, lane);
+  first[t] = t <= ranges ? w.first[t] : 0u;
+  if (t == 0) {
+    queued = 0;
+    if (ranges == MAX_RANGES) first[MAX_RANGES] = w.first[MAX_RANGES];
+  }
+  uint32_t all;
+  const uint32_t run = small_offsets<TINY_THREADS>((uint32_t)__builtin_amdgcn_readlane((int)inc, 63), wave_sum, &all) + inc - mine;
+  row[t] = run;                 // rows of the ranges before
+  if (t == 0) row[MAX_RANGES] = all;
+  __syncthreads();
+  if (blockIdx.x == 0 && t == 0) *count = (int32_t)all;
+  const int share = (int)(gridDim.x / (uint32_t)a.col_blocks), sh = (int)(blockIdx.x / (uint32_t)a.col_blocks);
+  const int r0 = (int)((int64_t)all * sh / share), r1 = (int)((int64_t)all * (sh + 1) / share);
+  auto range_of = [&](int r) {          // the range that holds row r0 + r: row[range] <= r0 + r < row[range + 1]
+    int lo = 0;
+#pragma unroll
+    for (int step = MAX_RANGES / 2; step; step >>= 1) lo += (int)row[lo + step] <= r0 + r ? step : 0;
+    return lo;
+  };
+  auto begin = [&](int r) {
+    const int k = range_of(r);
+    return (int)(first[k] + w.heads[first[k] + (uint32_t)(r0 + r) - row[k]]);
+  };
+  auto end = [&](int r) {
+    const int k = range_of(r);
+    const bool last = (uint32_t)(r0 + r) + 1 == row[k + 1];
+    return (int)(last ? first[k + 1] : first[k] + w.heads[first[k] + (uint32_t)(r0 + r) - row[k] + 1]);
+  };
+  small_sums<TINY_THREADS, TI, VEC>(
+      a, r1 - r0, begin, end, [&](int k) { return w.pos[k]; },
+      [&](int r, const float (&acc)[VEC], int col, int own) {
+        if (col == 0) {
+          const int k = range_of(r);
+          ids[r0 + r] = (int64_t)w.key[first[k] + (uint32_t)(r0 + r) - row[k]];
+        }
+        float f[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] = acc[j] * a.scale;
+        store_chunk<VEC, TO>((TO*)a.out + (int64_t)(r0 + r) * a.ld_out + col, f);
+      },
+      parts, queue, &queued);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -867,49 +1067,92 @@ int launch_sums(seg_args a, bool accumulate, hipStream_t stream) {
   return ORCA_OK;
 }
 
-int sum_by_type(int g_dtype, int out_dtype, const seg_args& a, bool accumulate, hipStream_t stream) {
-  if (out_dtype == ORCA_F32) {
-    if (g_dtype == ORCA_F32) return launch_sums<float, float>(a, accumulate, stream);
-    return g_dtype == ORCA_BF16 ? launch_sums<__bf16, float>(a, accumulate, stream) : launch_sums<_Float16, float>(a, accumulate, stream);
-  }
-  return g_dtype == ORCA_BF16 ? launch_sums<__bf16, __bf16>(a, accumulate, stream) : launch_sums<_Float16, _Float16>(a, accumulate, stream);
+bool is_small(int64_t n, int64_t width) { return n <= SMALL_N && n * width <= SMALL_VALUES; }
+bool maps(int64_t num_rows) { return num_rows <= 256LL * SMALL_MAP; }        // the workgroups of k_small can mark that many rows
+template <class T> void columns(small_args* a) {
+  constexpr int VEC = elems16<T>;
+  a->chunks = a->width < VEC ? a->width : (a->width + VEC - 1) / VEC;
+  a->log_l = log_lanes(a->chunks, 6);
+  a->col_blocks = (int)ceil_div64(a->chunks, 1 << a->log_l);
 }
-
-bool is_small(int64_t n, int64_t width, int64_t num_rows) {
-  return n <= SMALL_N && n * width <= SMALL_VALUES && num_rows <= 256LL * SMALL_MAP;
+int key_bits(int64_t num_rows) {
+  int bits = 1;
+  while ((num_rows >> bits) != 0) ++bits;
+  return bits;
 }
-template <class TI, class TO, int VEC, bool ACCUMULATE>
+template <int THREADS, class TI, class TO, int VEC, bool ACCUMULATE>
 int launch_small(small_args a, hipStream_t stream) {
   static bool seen[64] = {};
   if (orca_first_use_on_device(seen))
-    ORCA_HIP_TRY(hipFuncSetAttribute((const void*)k_small<TI, TO, VEC, ACCUMULATE>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                     small_layout(SMALL_N, MAX_DIGIT).bytes));
-  a.chunks = VEC == 1 ? a.width : (a.width + VEC - 1) / VEC;
-  a.log_l = log_lanes(a.chunks, 6);
-  a.col_blocks = (int)ceil_div64(a.chunks, 1 << a.log_l);
-  // workgroups: a distinct id per team, 128 KB of zeros or 65,536 rows each, at most one per CU (and one for each column block)
-  int64_t want = ceil_div64(a.n, SMALL_THREADS >> a.log_l) * a.col_blocks;
-  if (a.zero_rows) want = std::max({want, ceil_div64(a.src.num_rows * a.width * (int64_t)sizeof(TO), 131072), ceil_div64(a.src.num_rows, SMALL_MAP)});
+    ORCA_HIP_TRY(hipFuncSetAttribute((const void*)k_small<THREADS, TI, TO, VEC, ACCUMULATE>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                     small_layout(THREADS, THREADS * SMALL_ITEMS).bytes));
+  columns<TI>(&a);
+  // workgroups: four ids, 16 KB of zeros or 65,536 rows each, at most one per CU (and one for each column block)
+  int64_t want = ceil_div64(a.n, 4) * a.col_blocks;
+  if (a.zero_rows) want = std::max({want, ceil_div64(a.num_rows * a.width * (int64_t)sizeof(TO), 16384), ceil_div64(a.num_rows, SMALL_MAP)});
   const int64_t shares = std::max<int64_t>(1, ceil_div64(std::min<int64_t>(want, 256), a.col_blocks));
-  k_small<TI, TO, VEC, ACCUMULATE><<<(unsigned)(shares * a.col_blocks), SMALL_THREADS, small_layout(a.n, a.digit).bytes, stream>>>(a);
+  k_small<THREADS, TI, TO, VEC, ACCUMULATE>
+      <<<(unsigned)(shares * a.col_blocks), THREADS, small_layout(THREADS, a.n).bytes, stream>>>(a, key_bits(a.num_rows));
+  ORCA_LAUNCH_CHECK();
+  return ORCA_OK;
+}
+template <int THREADS, class TI, class TO>
+int small_dense(const small_args& a, bool accumulate, hipStream_t stream) {
+  constexpr int VEC = elems16<TI>;
+  if (a.width >= VEC) return accumulate ? launch_small<THREADS, TI, TO, VEC, true>(a, stream) : launch_small<THREADS, TI, TO, VEC, false>(a, stream);
+  return accumulate ? launch_small<THREADS, TI, TO, 1, true>(a, stream) : launch_small<THREADS, TI, TO, 1, false>(a, stream);
+}
+
+range_work range_layout(char* ws, int64_t n, int64_t* bytes) {
+  range_work w;
+  int64_t o = 0;
+  auto take = [&](int64_t b) { char* p = ws + o; o += (b + 255) / 256 * 256; return p; };
+  w.pos = (uint16_t*)take(2 * n);
+  w.heads = (uint16_t*)take(2 * n);
+  w.key = (uint32_t*)take(4 * n);
+  w.first = (uint32_t*)take(4 * (MAX_RANGES + 1));
+  w.distinct = (uint32_t*)take(4 * MAX_RANGES);
+  *bytes = o;
+  return w;
+}
+template <int THREADS> int launch_range_sort(const small_args& a, const range_work& w, int ranges, hipStream_t stream) {
+  static bool seen[64] = {};
+  if (orca_first_use_on_device(seen))
+    ORCA_HIP_TRY(hipFuncSetAttribute((const void*)k_range_sort<THREADS>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                     small_layout(THREADS, THREADS * SMALL_ITEMS).bytes));
+  k_range_sort<THREADS><<<(unsigned)ranges, THREADS, small_layout(THREADS, a.n).bytes, stream>>>(a, w);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
 template <class TI, class TO>
-int small_typed(const small_args& a, bool accumulate, hipStream_t stream) {
+int small_rows(small_args a, char* ws, int64_t* ids, int32_t* count, hipStream_t stream) {
   constexpr int VEC = elems16<TI>;
-  if (a.width >= VEC) return accumulate ? launch_small<TI, TO, VEC, true>(a, stream) : launch_small<TI, TO, VEC, false>(a, stream);
-  return accumulate ? launch_small<TI, TO, 1, true>(a, stream) : launch_small<TI, TO, 1, false>(a, stream);
+  columns<TI>(&a);
+  int64_t bytes;
+  const range_work w = range_layout(ws, a.n, &bytes);
+  const int ranges = (int)std::min<int64_t>(MAX_RANGES, ceil_div64(a.n, 4));
+  if (int rc = a.n <= TINY_N ? launch_range_sort<TINY_THREADS>(a, w, ranges, stream) : launch_range_sort<SMALL_THREADS>(a, w, ranges, stream)) return rc;
+  // a run per team and workgroup, at most two workgroups per CU (and one for each column block)
+  const int64_t shares = std::max<int64_t>(1, std::min(ceil_div64(a.n, TINY_THREADS >> a.log_l), ceil_div64(512, a.col_blocks)));
+  const unsigned grid = (unsigned)(shares * a.col_blocks);
+  if (a.width >= VEC) k_range_sums<TI, TO, VEC><<<grid, TINY_THREADS, 0, stream>>>(a, w, ranges, ids, count);
+  else k_range_sums<TI, TO, 1><<<grid, TINY_THREADS, 0, stream>>>(a, w, ranges, ids, count);
+  ORCA_LAUNCH_CHECK();
+  return ORCA_OK;
 }
-int small_by_type(int g_dtype, int out_dtype, small_args a, bool accumulate, hipStream_t stream) {
-  const sort_plan s = plan_sort(a.n, a.src.num_rows);
-  a.passes = s.passes;
-  a.digit = s.digit;
-  if (out_dtype == ORCA_F32) {
-    if (g_dtype == ORCA_F32) return small_typed<float, float>(a, accumulate, stream);
-    return g_dtype == ORCA_BF16 ? small_typed<__bf16, float>(a, accumulate, stream) : small_typed<_Float16, float>(a, accumulate, stream);
-  }
-  return g_dtype == ORCA_BF16 ? small_typed<__bf16, __bf16>(a, accumulate, stream) : small_typed<_Float16, _Float16>(a, accumulate, stream);
+
+// f(gradient element, output element) for the pairs of types that check_gradient lets through
+template <class F> int by_types(int g_dtype, int out_dtype, F f) {
+  if (g_dtype == ORCA_F32) return f(float{}, float{});
+  if (g_dtype == ORCA_BF16) return out_dtype == ORCA_F32 ? f(__bf16{}, float{}) : f(__bf16{}, __bf16{});
+  return out_dtype == ORCA_F32 ? f(_Float16{}, float{}) : f(_Float16{}, _Float16{});
+}
+
+int64_t workspace_bytes_of(int64_t n, int64_t width, int64_t num_rows) {
+  if (!is_small(n, width)) return layout(n, width, num_rows).bytes;
+  int64_t bytes;
+  range_layout(nullptr, n, &bytes);
+  return maps(num_rows) ? bytes : std::max(bytes, layout(n, width, num_rows).bytes);
 }
 
 int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, const int64_t* idx64, const int32_t* idx32, int64_t n, int64_t width,
@@ -922,8 +1165,8 @@ int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, co
   if (n == 0) return ORCA_OK;
   ORCA_REQUIRE(g && (idx64 != nullptr) != (idx32 != nullptr), "%s: null gradient, or not exactly one list of ids", who);
   ORCA_REQUIRE(ld_g >= 0, "%s: negative row stride", who);
-  ORCA_REQUIRE(workspace && workspace_bytes >= layout(n, width, num_rows).bytes, "%s: the workspace holds %lld of %lld bytes", who,
-               (long long)workspace_bytes, (long long)layout(n, width, num_rows).bytes);
+  ORCA_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(n, width, num_rows), "%s: the workspace holds %lld of %lld bytes", who,
+               (long long)workspace_bytes, (long long)workspace_bytes_of(n, width, num_rows));
   return ORCA_OK;
 }
 
@@ -976,7 +1219,7 @@ ORCA_API int orca_embedding_forward(const void* table, int dtype, int64_t n_rows
 
 ORCA_API int64_t orca_embedding_backward_workspace_bytes(int64_t n, int64_t width, int64_t num_rows) {
   if (n < 0 || n >= (1LL << 31) || width < 1 || width > MAX_WIDTH || num_rows < 0 || num_rows >= (1LL << 31) - 1) return -1;
-  return layout(n, width, num_rows).bytes;
+  return workspace_bytes_of(n, width, num_rows);
 }
 
 ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64_t ld_grad, const int64_t* idx64, const int32_t* idx32, int64_t n,
@@ -1004,11 +1247,12 @@ ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64
     ORCA_LAUNCH_CHECK();
     return ORCA_OK;
   }
-  if (is_small(n, width, num_rows)) {
-    small_args a{{idx64, idx32, nullptr, n, num_rows, padding_idx}, grad_out, ld_grad, ld_table, grad_table, nullptr, nullptr, (int)n, (int)width};
-    a.zero_rows = !accumulate;
-    a.scale = scale;
-    return small_by_type(grad_dtype, table_dtype, a, accumulate != 0, stream);
+  if (is_small(n, width) && (accumulate || maps(num_rows))) {
+    const small_args a{idx64, idx32, num_rows, padding_idx, grad_out, ld_grad, ld_table, grad_table, (int)n, (int)width, 0, 0, 0, !accumulate, scale};
+    return by_types(grad_dtype, table_dtype, [&](auto gi, auto go) {
+      return n <= TINY_N ? small_dense<TINY_THREADS, decltype(gi), decltype(go)>(a, accumulate != 0, stream)
+                         : small_dense<SMALL_THREADS, decltype(gi), decltype(go)>(a, accumulate != 0, stream);
+    });
   }
   const work_layout l = layout(n, width, num_rows);
   char* ws = (char*)workspace;
@@ -1016,7 +1260,8 @@ ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64
   if (int rc = sort_positions(idx64, idx32, n, num_rows, padding_idx, ws, l, fill, pieces, &s, stream)) return rc;
   seg_args a{grad_out, ld_grad, n, ld_table, s, nullptr, grad_table, (float*)(ws + l.part), (int)width, 0, 0, window_of(n, width), 0,
              (uint32_t)num_rows, scale};
-  return sum_by_type(grad_dtype, table_dtype, a, accumulate != 0, stream);
+  return by_types(grad_dtype, table_dtype,
+                  [&](auto gi, auto go) { return launch_sums<decltype(gi), decltype(go)>(a, accumulate != 0, stream); });
 }
 
 ORCA_API int orca_embedding_backward_rows(const void* grad_out, int grad_dtype, int64_t ld_grad, const int64_t* idx64, const int32_t* idx32, int64_t n,
@@ -1028,10 +1273,10 @@ ORCA_API int orca_embedding_backward_rows(const void* grad_out, int grad_dtype, 
     return rc;
   ORCA_REQUIRE(count && (n == 0 || (ids && rows)), "orca_embedding_backward_rows: null output");
   if (n == 0) return orca_fill_i32(count, 1, 0, stream_);
-  if (is_small(n, width, num_rows)) {
-    small_args a{{idx64, idx32, nullptr, n, num_rows, padding_idx}, grad_out, ld_grad, width, rows, ids, count, (int)n, (int)width};
-    a.scale = scale;
-    return small_by_type(grad_dtype, rows_dtype, a, false, stream);
+  if (is_small(n, width)) {
+    const small_args a{idx64, idx32, num_rows, padding_idx, grad_out, ld_grad, width, rows, (int)n, (int)width, 0, 0, 0, 0, scale};
+    return by_types(grad_dtype, rows_dtype,
+                    [&](auto gi, auto go) { return small_rows<decltype(gi), decltype(go)>(a, (char*)workspace, ids, count, stream); });
   }
   const work_layout l = layout(n, width, num_rows);
   char* ws = (char*)workspace;
@@ -1044,5 +1289,5 @@ ORCA_API int orca_embedding_backward_rows(const void* grad_out, int grad_dtype, 
   k_rank<<<tiles, SORT_THREADS, 0, stream>>>(s, n, (uint32_t)num_rows, (const uint32_t*)(ws + l.heads), rank, ids, count);
   ORCA_LAUNCH_CHECK();
   seg_args a{grad_out, ld_grad, n, width, s, rank, rows, (float*)(ws + l.part), (int)width, 0, 0, window_of(n, width), 0, (uint32_t)num_rows, scale};
-  return sum_by_type(grad_dtype, rows_dtype, a, false, stream);
+  return by_types(grad_dtype, rows_dtype, [&](auto gi, auto go) { return launch_sums<decltype(gi), decltype(go)>(a, false, stream); });
 }
