@@ -1,71 +1,122 @@
 // The global 2-norm of a list of gradient tensors and their scaling to a largest norm (torch.nn.utils.clip_grad_norm_'s formula):
 //   N = sqrt(sum g^2),  c = min(1, max_norm / (N + 1e-6)),  g <- c * g
-// Two launches per GROUP_MAX tensors, no atomics and no host read: k_norm_partial leaves one fp64 sum per workgroup, and every
-// workgroup of k_clip adds those sums up in the same order before it scales its share.  Squares and sums are fp64: neither
-// overflows nor vanishes for any fp32 input, and the conversion is hidden behind the loads (4.5 elements per clock and CU at the
+// Two launches per list, no atomics and no host read: k_norm_partial leaves one fp64 sum per workgroup, and every workgroup of k_clip
+// adds those sums up in the same order (while its first piece is on its way) before it scales its share.  Squares and sums are fp64:
+// neither overflows nor vanishes for any fp32 input, and the conversions hide behind the loads (4.5 elements per clock and CU at the
 // HBM rate for 16-bit gradients).
+//   A list travels in the kernel's arguments, under 4 KB: 12 bytes per tensor (20 with flat buffers), so that a few hundred tensors
+// are one launch.  With a search by scalar loads through 41 bytes per tensor, k_norm_partial took 6.4 us for 32 tensors of 2.9 MB.
 #include <algorithm>
 #include "elem.h"
 
 namespace {
-constexpr int GROUP_MAX = 96;         // tensors per launch: the group travels in the kernel's arguments (under 4 KB)
-constexpr int TILE = 8192;            // elements a workgroup takes at a time
+constexpr int PIECE = 16384, SMALL_PIECE = 4096;        // bytes a workgroup takes at a time: short lists spread over more workgroups
+// Flat buffers from here on: gradients read and products written past the caches (non-temporal).  Both ways measured, fp32 list, us:
+// 60 MB 33.1 against 31.6 with plain accesses, 120 MB 59.7 (71.9), 300 MB 142 (174), 1 GB 484 (552).
+constexpr int64_t STREAM_BYTES = 100000000;
 constexpr int PARTS = 2048;           // most partial sums of a call
+constexpr int SPARSE_MAX = 8;         // row-sparse tensors per launch
 
-struct grad_group {
-  int n;
-  int first[GROUP_MAX + 1];           // first tile of each tensor
-  uint8_t dtype[GROUP_MAX];
-  int32_t width[GROUP_MAX];           // of a row-sparse tensor
-  const int32_t* rows[GROUP_MAX];     // its device count, or null
-  void* g[GROUP_MAX];
-  void* out[GROUP_MAX];               // k_clip: where the products go
-  int64_t size[GROUP_MAX];
+struct sparse_grad {
+  const int32_t* rows;                // the device count
+  int32_t width, dtype;
 };
-static_assert(sizeof(grad_group) <= 4000, "kernel arguments");
+// Tensor t: its address in the low 48 bits, the bytes of its last piece / 2 - 1 in the next 13, 1 for a row-sparse one, its type in the top 2
+// (row-sparse: its number in `sparse` is in `which`).
+template <int N, bool FLAT> struct grad_list {
+  int n, n_sparse;
+  uint64_t at[N];
+  int first[N + 1];                   // first piece of each tensor
+  int which[SPARSE_MAX];              // the tensors that are row-sparse
+  sparse_grad sparse[SPARSE_MAX];
+  int64_t to[FLAT ? N : 1];           // flat: where the tensor begins in its type's buffer, in elements
+  char* flat[3];
+};
+typedef grad_list<300, false> in_place_list;
+typedef grad_list<180, true> flat_list;
+static_assert(sizeof(in_place_list) <= 4000 && sizeof(flat_list) <= 4000, "kernel arguments");
 
-// the tensor that tile belongs to (uniform), its size now, and the tile's first element
-__device__ __forceinline__ int locate(const grad_group& grp, int tile, int64_t* base, int64_t* size) {
-  int lo = 0, hi = grp.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (tile >= grp.first[mid]) lo = mid; else hi = mid;
+struct piece { char* p; int64_t offset; int len, dtype, tensor; };       // offset: bytes from the tensor's beginning
+// the lanes hold the first pieces of all tensors: those at or before a piece are counted in one go
+template <class L> struct locator {
+  static constexpr int K = (int)(sizeof(L::first) / 4 + 62) / 64;
+  int first[K];
+  __device__ __forceinline__ explicit locator(const L& list) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 0; k < K; ++k) first[k] = 64 * k + lane < list.n ? list.first[64 * k + lane] : 0x7fffffff;
   }
-  *base = (int64_t)(tile - grp.first[lo]) * TILE;
-  int64_t s = grp.size[lo];
-  if (grp.rows[lo]) {
-    const int64_t have = (int64_t)*grp.rows[lo] * grp.width[lo];
-    s = have < s ? (have > 0 ? have : 0) : s;
+  __device__ __forceinline__ piece find(const L& list, int i, int bytes) const {
+    int t = -1;
+#pragma unroll
+    for (int k = 0; k < K; ++k) t += __popcll(__ballot(first[k] <= i));
+    t = __builtin_amdgcn_readfirstlane(t);
+    const uint64_t at = list.at[t];
+    const int begin = list.first[t], end = list.first[t + 1];
+    piece q;
+    q.tensor = t;
+    q.p = reinterpret_cast<char*>(at & 0xffffffffffffULL);
+    q.dtype = (int)(at >> 62);
+    q.offset = (int64_t)(i - begin) * bytes;
+    q.len = i + 1 == end ? (((int)(at >> 48) & 0x1fff) + 1) * 2 : bytes;
+    if ((at >> 61) & 1) {
+      for (int s = 0; s < list.n_sparse; ++s)
+        if (list.which[s] == t) {
+          const int rows = *list.sparse[s].rows;
+          const int64_t have = (int64_t)(rows > 0 ? rows : 0) * list.sparse[s].width * (q.dtype == ORCA_F32 ? 4 : 2) - q.offset;
+          q.len = have < q.len ? (have > 0 ? (int)have : 0) : q.len;
+        }
+    }
+    return q;
   }
-  *size = s;
-  return lo;
-}
+};
 
-template <class T>
-__device__ __forceinline__ double tile_squares(const T* __restrict__ g, int64_t base, int64_t size) {
-  constexpr int VEC = elems16<T>, STEPS = TILE / (256 * VEC);
+template <class T, int STEPS>
+__device__ __forceinline__ double squares(const u32x4 (&r)[STEPS], const piece& q) {
   double acc = 0.0;
-  if (base + TILE <= size) {
-    u32x4 r[STEPS];
+  auto add = [&](float f) { acc = fma((double)f, (double)f, acc); };
 #pragma unroll
-    for (int k = 0; k < STEPS; ++k) r[k] = load16(g + base + (threadIdx.x + 256 * k) * VEC);
-#pragma unroll
-    for (int k = 0; k < STEPS; ++k) {
-      float f[VEC];
+  for (int k = 0; k < STEPS; ++k) {
+    const int b = ((int)threadIdx.x + 256 * k) * 16;
+    if (b + 16 <= q.len) {
+      float f[elems16<T>];
       unpack16<T>(r[k], f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const double d = (double)f[j];
-        acc = fma(d, d, acc);
-      }
-    }
-  } else {
-    for (int64_t i = base + threadIdx.x; i < size; i += 256) {
-      const double d = (double)(float)g[i];
-      acc = fma(d, d, acc);
+      for (int j = 0; j < elems16<T>; ++j) add(f[j]);
+    } else {
+      for (int e = b; e < q.len; e += (int)sizeof(T)) add((float)*reinterpret_cast<const T*>(q.p + q.offset + e));
     }
   }
   return acc;
+}
+template <bool STREAMS, class T, int STEPS>
+__device__ __forceinline__ void scale(const u32x4 (&r)[STEPS], const piece& q, char* out, float c) {
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int b = ((int)threadIdx.x + 256 * k) * 16;
+    if (b + 16 <= q.len) {
+      float f[elems16<T>];
+      unpack16<T>(r[k], f);
+#pragma unroll
+      for (int j = 0; j < elems16<T>; ++j) f[j] *= c;
+      if constexpr (STREAMS) __builtin_nontemporal_store(pack16<T>(f), reinterpret_cast<u32x4_any*>(out + b));
+      else store16(out + b, pack16<T>(f));
+    } else {
+      for (int e = b; e < q.len; e += (int)sizeof(T))
+        *reinterpret_cast<T*>(out + e) = (T)((float)*reinterpret_cast<const T*>(q.p + q.offset + e) * c);
+    }
+  }
+}
+template <bool STREAMS, int STEPS>
+__device__ __forceinline__ void request(u32x4 (&r)[STEPS], const piece& q) {
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int b = ((int)threadIdx.x + 256 * k) * 16;
+    if (b + 16 <= q.len) {
+      if constexpr (STREAMS) r[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(q.p + q.offset + b));
+      else r[k] = load16(q.p + q.offset + b);
+    }
+  }
 }
 
 // sum over the workgroup's 256 threads, the same bits in every thread
@@ -77,17 +128,21 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-__global__ __launch_bounds__(256) void k_norm_partial(grad_group grp, double* __restrict__ part) {
+// The pieces are taken from the last to the first: what was read last is still in the 256 MB last-level cache when k_clip begins.
+template <int BYTES>
+__global__ __launch_bounds__(256) void k_norm_partial(in_place_list list, double* __restrict__ part) {
+  constexpr int STEPS = BYTES / 4096;
   __shared__ double lds[4];
+  const locator<in_place_list> where(list);
+  const int pieces = list.first[list.n];
   double acc = 0.0;
-  const int tiles = grp.first[grp.n];
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    int64_t base, size;
-    const int t = locate(grp, tile, &base, &size);
-    if (base >= size) continue;
-    if (grp.dtype[t] == ORCA_F32) acc += tile_squares((const float*)grp.g[t], base, size);
-    else if (grp.dtype[t] == ORCA_BF16) acc += tile_squares((const __bf16*)grp.g[t], base, size);
-    else acc += tile_squares((const _Float16*)grp.g[t], base, size);
+  for (int i = pieces - 1 - (int)blockIdx.x; i >= 0; i -= (int)gridDim.x) {
+    const piece q = where.find(list, i, BYTES);
+    u32x4 r[STEPS];
+    request<false>(r, q);
+    if (q.dtype == ORCA_F32) acc += squares<float>(r, q);
+    else if (q.dtype == ORCA_BF16) acc += squares<__bf16>(r, q);
+    else acc += squares<_Float16>(r, q);
   }
   const double s = block_sum(acc, lds);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -95,12 +150,14 @@ __global__ __launch_bounds__(256) void k_norm_partial(grad_group grp, double* __
 
 // the coefficient from the partial sums: every workgroup adds them in the same order
 __device__ __forceinline__ float coefficient(const double* __restrict__ part, int parts, double max_norm, double* lds, double* norm) {
-  double acc = 0.0;
+  double v[PARTS / 256], acc = 0.0;
 #pragma unroll
   for (int k = 0; k < PARTS / 256; ++k) {
     const int i = threadIdx.x + 256 * k;
-    acc += i < parts ? part[i] : 0.0;
+    v[k] = i < parts ? part[i] : 0.0;
   }
+#pragma unroll
+  for (int k = 0; k < PARTS / 256; ++k) acc += v[k];
   *norm = sqrt(block_sum(acc, lds));
   const double c = max_norm / (*norm + 1e-6);
   return c > 1.0 ? 1.0f : (float)c;       // (a NaN stays one)
@@ -117,100 +174,128 @@ __global__ __launch_bounds__(256) void k_norm_finish(const double* __restrict__ 
   }
 }
 
-template <class T>
-__device__ __forceinline__ void tile_scale(const T* g, T* out, int64_t base, int64_t size, float c) {
-  constexpr int VEC = elems16<T>, STEPS = TILE / (256 * VEC);
-  if (base + TILE <= size) {
-    u32x4 r[STEPS];
-#pragma unroll
-    for (int k = 0; k < STEPS; ++k) r[k] = load16(g + base + (threadIdx.x + 256 * k) * VEC);
-#pragma unroll
-    for (int k = 0; k < STEPS; ++k) {
-      float f[VEC];
-      unpack16<T>(r[k], f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] *= c;
-      store16(out + base + (threadIdx.x + 256 * k) * VEC, pack16<T>(f));
-    }
-  } else {
-    for (int64_t i = base + threadIdx.x; i < size; i += 256) out[i] = (T)((float)g[i] * c);
-  }
-}
-
-__global__ __launch_bounds__(256) void k_clip(grad_group grp, const double* __restrict__ part, int parts, double max_norm, int in_place,
-                                              float* __restrict__ norm) {
+template <int BYTES, bool STREAMS, class L, bool FLAT>
+__global__ __launch_bounds__(256) void k_clip(L list, const double* __restrict__ part, int parts, double max_norm, float* __restrict__ norm) {
+  constexpr int STEPS = BYTES / 4096;
   __shared__ double lds[4];
+  const locator<L> where(list);
+  const int pieces = list.first[list.n];
+  int i = blockIdx.x;
+  piece q = where.find(list, i, BYTES);                   // (there are at least as many pieces as workgroups)
+  u32x4 r[STEPS];
+  request<STREAMS>(r, q);
   double n;
   const float c = coefficient(part, parts, max_norm, lds, &n);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-  if (in_place && c == 1.0f) return;
-  const int tiles = grp.first[grp.n];
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    int64_t base, size;
-    const int t = locate(grp, tile, &base, &size);
-    if (base >= size) continue;
-    if (grp.dtype[t] == ORCA_F32) tile_scale((const float*)grp.g[t], (float*)grp.out[t], base, size, c);
-    else if (grp.dtype[t] == ORCA_BF16) tile_scale((const __bf16*)grp.g[t], (__bf16*)grp.out[t], base, size, c);
-    else tile_scale((const _Float16*)grp.g[t], (_Float16*)grp.out[t], base, size, c);
+  if (!FLAT && c == 1.0f) return;
+  for (;;) {
+    char* out = q.p + q.offset;
+    if constexpr (FLAT) out = list.flat[q.dtype] + list.to[q.tensor] * (q.dtype == ORCA_F32 ? 4 : 2) + q.offset;
+    if (q.dtype == ORCA_F32) scale<STREAMS, float>(r, q, out, c);
+    else if (q.dtype == ORCA_BF16) scale<STREAMS, __bf16>(r, q, out, c);
+    else scale<STREAMS, _Float16>(r, q, out, c);
+    i += (int)gridDim.x;
+    if (i >= pieces) break;
+    q = where.find(list, i, BYTES);
+    request<STREAMS>(r, q);
   }
 }
 
-int check_list(const char* who, int n, void* const* grads, const int64_t* sizes, const uint8_t* dtypes, const int32_t* const* rows, const int32_t* widths,
-               double max_norm, const float* norm, const void* workspace, int64_t* tiles) {
-  ORCA_REQUIRE(n >= 0 && n <= 65536 && norm && workspace && (n == 0 || (grads && sizes && dtypes)) && (!rows || widths), "%s: null argument, or not 0 to 65536 tensors", who);
+struct host_list {
+  int n;
+  void* const* grads;
+  const int64_t* sizes;
+  const uint8_t* dtypes;
+  const int32_t* const* rows;
+  const int32_t* widths;
+  int piece;                          // bytes, for the whole call
+  int64_t pieces;
+};
+int64_t bytes_of(const host_list& h, int i) { return h.sizes[i] * (h.dtypes[i] == ORCA_F32 ? 4 : 2); }
+
+int check_list(const char* who, host_list* h, double max_norm, const float* norm, const void* workspace) {
+  ORCA_REQUIRE(h->n >= 0 && h->n <= 65536 && norm && workspace && (h->n == 0 || (h->grads && h->sizes && h->dtypes)) && (!h->rows || h->widths),
+               "%s: null argument, or not 0 to 65536 tensors", who);
   ORCA_REQUIRE(max_norm >= 0.0, "%s: max_norm %g (not negative, not NaN)", who, max_norm);
-  *tiles = 0;
-  for (int i = 0; i < n; ++i) {
-    ORCA_REQUIRE(sizes[i] >= 0 && sizes[i] < (1LL << 40) && (sizes[i] == 0 || grads[i]), "%s: tensor %d: null, or a bad size", who, i);
-    ORCA_REQUIRE(dtypes[i] <= ORCA_F16, "%s: tensor %d: unknown type %d", who, i, dtypes[i]);
-    ORCA_REQUIRE(!rows || !rows[i] || widths[i] >= 1, "%s: tensor %d: width %d", who, i, rows && rows[i] ? widths[i] : 0);
-    *tiles += ceil_div64(sizes[i], TILE);
+  int64_t total = 0;
+  for (int i = 0; i < h->n; ++i) {
+    ORCA_REQUIRE(h->sizes[i] >= 0 && h->sizes[i] < (1LL << 40) && (h->sizes[i] == 0 || h->grads[i]), "%s: tensor %d: null, or a bad size", who, i);
+    ORCA_REQUIRE(h->dtypes[i] <= ORCA_F16, "%s: tensor %d: unknown type %d", who, i, h->dtypes[i]);
+    ORCA_REQUIRE(!h->rows || !h->rows[i] || h->widths[i] >= 1, "%s: tensor %d: width %d", who, i, h->rows && h->rows[i] ? h->widths[i] : 0);
+    ORCA_REQUIRE(((uint64_t)(uintptr_t)h->grads[i] >> 48) == 0 && ((uintptr_t)h->grads[i] & 1) == 0, "%s: tensor %d: not a device address", who, i);
+    total += bytes_of(*h, i);
   }
-  ORCA_REQUIRE(*tiles < (1LL << 31), "%s: too many elements for one call", who);
+  // small pieces up to four workgroups per CU of them
+  h->piece = total <= 1024LL * SMALL_PIECE ? SMALL_PIECE : PIECE;
+  h->pieces = 0;
+  for (int i = 0; i < h->n; ++i) h->pieces += ceil_div64(bytes_of(*h, i), h->piece);
+  ORCA_REQUIRE(h->pieces < (1LL << 31), "%s: too many elements for one call", who);
   return ORCA_OK;
 }
 
-// calls f(group, its tiles) for each GROUP_MAX tensors that hold anything
-template <class F>
-int each_group(int n, void* const* grads, const int64_t* sizes, const uint8_t* dtypes, const int32_t* const* rows, const int32_t* widths,
-               void* const* flat, F f) {
-  int64_t used[3] = {0, 0, 0};
-  for (int i = 0; i < n;) {
-    grad_group grp{};
-    int64_t tiles = 0;
-    for (; i < n && grp.n < GROUP_MAX; ++i) {
-      const int k = grp.n, dt = dtypes[i];
-      if (sizes[i] == 0) continue;
-      grp.first[k] = (int)tiles;
-      grp.dtype[k] = (uint8_t)dt;
-      grp.rows[k] = rows ? rows[i] : nullptr;
-      grp.width[k] = grp.rows[k] ? widths[i] : 0;
-      grp.g[k] = grads[i];
-      grp.out[k] = flat ? (char*)flat[dt] + used[dt] : grads[i];
-      grp.size[k] = sizes[i];
-      used[dt] += sizes[i] * (dt == ORCA_F32 ? 4 : 2);
-      tiles += ceil_div64(sizes[i], TILE);
-      grp.first[++grp.n] = (int)tiles;
+// The list from tensor *i on, as much of it as a launch takes.  `to`: elements of each type so far (flat buffers), moved on.
+template <class L, bool FLAT> void take(const host_list& h, int* i, int64_t* to, L* list) {
+  constexpr int N = (int)(sizeof(L::at) / 8);
+  list->n = list->n_sparse = 0;
+  int64_t pieces = 0;
+  for (; *i < h.n && list->n < N; ++*i) {
+    if (h.sizes[*i] == 0) continue;
+    const int t = list->n, dt = h.dtypes[*i];
+    const bool sparse = h.rows && h.rows[*i];
+    if (sparse && list->n_sparse == SPARSE_MAX) break;
+    const int64_t bytes = bytes_of(h, *i), mine = ceil_div64(bytes, h.piece);
+    const uint64_t tail = (uint64_t)(bytes - (mine - 1) * h.piece);
+    list->at[t] = (uint64_t)(uintptr_t)h.grads[*i] | (tail / 2 - 1) << 48 | (uint64_t)sparse << 61 | (uint64_t)dt << 62;
+    if (sparse) {
+      list->which[list->n_sparse] = t;
+      list->sparse[list->n_sparse++] = sparse_grad{h.rows[*i], h.widths[*i], dt};
     }
-    if (grp.n) {
-      if (int rc = f(grp, tiles)) return rc;
+    if constexpr (FLAT) {
+      list->to[t] = to[dt];
+      to[dt] += h.sizes[*i];
     }
+    list->first[t] = (int)pieces;
+    pieces += mine;
+    list->first[t + 1] = (int)pieces;
+    list->n = t + 1;
   }
-  return ORCA_OK;
 }
 
-// k_norm_partial over the list: *parts sums, at most PARTS (each group gets its share of them)
-int partial_sums(int n, void* const* grads, const int64_t* sizes, const uint8_t* dtypes, const int32_t* const* rows, const int32_t* widths, int64_t tiles,
-                 double* part, int* parts, hipStream_t stream) {
+// k_norm_partial over the list: *parts sums, at most PARTS (each launch gets its share of them)
+int partial_sums(const host_list& h, double* part, int* parts, hipStream_t stream) {
   *parts = 0;
-  const int64_t room = PARTS - ceil_div64(n, GROUP_MAX);
-  return each_group(n, grads, sizes, dtypes, rows, widths, nullptr, [&](const grad_group& grp, int64_t mine) {
-    const int64_t grid = std::min(mine, mine * room / tiles + 1);
-    k_norm_partial<<<(unsigned)grid, 256, 0, stream>>>(grp, part + *parts);
-    *parts += (int)grid;
+  const int64_t launches = ceil_div64(h.n, SPARSE_MAX), room = PARTS - std::min<int64_t>(launches, PARTS / 2);
+  for (int i = 0; i < h.n;) {
+    in_place_list list;
+    take<in_place_list, false>(h, &i, nullptr, &list);
+    if (list.n == 0) continue;
+    const int64_t mine = list.first[list.n], grid = std::min({mine, mine * room / h.pieces + 1, (int64_t)(PARTS - *parts)});
+    ORCA_REQUIRE(grid > 0, "orca_grad_norm: too many row-sparse gradients for one call");
+    if (h.piece == PIECE) k_norm_partial<PIECE><<<(unsigned)grid, 256, 0, stream>>>(list, part + *parts);
+    else k_norm_partial<SMALL_PIECE><<<(unsigned)grid, 256, 0, stream>>>(list, part + *parts);
     ORCA_LAUNCH_CHECK();
-    return ORCA_OK;
-  });
+    *parts += (int)grid;
+  }
+  return ORCA_OK;
+}
+
+template <class L, bool FLAT>
+int clip(const host_list& h, void* const* flat, const double* part, int parts, double max_norm, float* norm, hipStream_t stream) {
+  int64_t to[3] = {0, 0, 0};
+  for (int i = 0; i < h.n;) {
+    L list;
+    take<L, FLAT>(h, &i, to, &list);
+    if (list.n == 0) continue;
+    if constexpr (FLAT)
+      for (int k = 0; k < 3; ++k) list.flat[k] = (char*)flat[k];
+    const unsigned grid = (unsigned)std::min(list.first[list.n], 2048);
+    if (h.piece == SMALL_PIECE) k_clip<SMALL_PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, part, parts, max_norm, norm);
+    else if (FLAT && h.pieces * h.piece > STREAM_BYTES) k_clip<PIECE, FLAT, L, FLAT><<<grid, 256, 0, stream>>>(list, part, parts, max_norm, norm);
+    else k_clip<PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, part, parts, max_norm, norm);
+    ORCA_LAUNCH_CHECK();
+    norm = nullptr;             // (the first launch writes it)
+  }
+  return ORCA_OK;
 }
 }  // namespace
 
@@ -219,10 +304,10 @@ ORCA_API int64_t orca_grad_norm_workspace_bytes(void) { return PARTS * 8; }
 ORCA_API int orca_grad_norm(int n, void* const* grads, const int64_t* sizes, const uint8_t* dtypes, const int32_t* const* rows, const int32_t* widths,
                             double max_norm, float* norm, float* coef, void* workspace, void* stream_) {
   hipStream_t stream = (hipStream_t)stream_;
-  int64_t tiles = 0;
+  host_list h{n, grads, sizes, dtypes, rows, widths, 0, 0};
   int parts = 0;
-  if (int rc = check_list("orca_grad_norm", n, grads, sizes, dtypes, rows, widths, max_norm, norm, workspace, &tiles)) return rc;
-  if (int rc = partial_sums(n, grads, sizes, dtypes, rows, widths, tiles, (double*)workspace, &parts, stream)) return rc;
+  if (int rc = check_list("orca_grad_norm", &h, max_norm, norm, workspace)) return rc;
+  if (int rc = partial_sums(h, (double*)workspace, &parts, stream)) return rc;
   k_norm_finish<<<1, 256, 0, stream>>>((const double*)workspace, parts, max_norm, norm, coef);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
@@ -231,21 +316,17 @@ ORCA_API int orca_grad_norm(int n, void* const* grads, const int64_t* sizes, con
 ORCA_API int orca_clip_grads(int n, void* const* grads, const int64_t* sizes, const uint8_t* dtypes, const int32_t* const* rows, const int32_t* widths,
                              double max_norm, void* const* flat, float* norm, void* workspace, void* stream_) {
   hipStream_t stream = (hipStream_t)stream_;
-  int64_t tiles = 0;
+  host_list h{n, grads, sizes, dtypes, rows, widths, 0, 0};
   int parts = 0;
-  if (int rc = check_list("orca_clip_grads", n, grads, sizes, dtypes, rows, widths, max_norm, norm, workspace, &tiles)) return rc;
+  if (int rc = check_list("orca_clip_grads", &h, max_norm, norm, workspace)) return rc;
   for (int i = 0; flat && i < n; ++i) ORCA_REQUIRE(sizes[i] == 0 || flat[dtypes[i]], "orca_clip_grads: no flat buffer for type %d", dtypes[i]);
-  if (int rc = partial_sums(n, grads, sizes, dtypes, rows, widths, tiles, (double*)workspace, &parts, stream)) return rc;
-  if (tiles == 0) {
-    k_norm_finish<<<1, 256, 0, stream>>>((const double*)workspace, 0, max_norm, norm, nullptr);
+  if (int rc = partial_sums(h, (double*)workspace, &parts, stream)) return rc;
+  const double* part = (const double*)workspace;
+  if (h.pieces == 0) {
+    k_norm_finish<<<1, 256, 0, stream>>>(part, 0, max_norm, norm, nullptr);
     ORCA_LAUNCH_CHECK();
     return ORCA_OK;
   }
-  float* norm_out = norm;         // the first group's launch writes it
-  return each_group(n, grads, sizes, dtypes, rows, widths, flat, [&](const grad_group& grp, int64_t mine) {
-    k_clip<<<(unsigned)std::min<int64_t>(mine, 2048), 256, 0, stream>>>(grp, (const double*)workspace, parts, max_norm, flat == nullptr, norm_out);
-    norm_out = nullptr;
-    ORCA_LAUNCH_CHECK();
-    return ORCA_OK;
-  });
+  return flat ? clip<flat_list, true>(h, flat, part, parts, max_norm, norm, stream)
+              : clip<in_place_list, false>(h, flat, part, parts, max_norm, norm, stream);
 }
