@@ -3,11 +3,13 @@ gfx950.  Run here on the CPU container (hipcc cross-compiles); the .so travels t
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "liborca_hip.so")
+HOST = os.path.join(HERE, "_host.so")      # csrc/bind.cpp: torch tensors -> C ABI for the calls where the host's time counts
 SOURCES = ["csr.hip", "tgat.hip", "tgat_bwd.hip", "gru_bwd.hip", "gru.hip", "state.hip", "plan.hip", "plan_dev.hip", "engine.hip", "optim.hip", "clip.hip", "embedding.hip", "decoder.hip"]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-Wall",
          "-Wno-unused-result", "-Wno-unused-function"]
@@ -45,8 +47,18 @@ def build(force=False, verbose=False):
       print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
 
+  bind = os.path.join(CSRC, "bind.cpp")
+  host = []
+  if force or _stale(HOST, [bind, os.path.join(inc, "orca_hip.h")]):
+    import torch      # (headers and libraries of the torch that will load it)
+    t = os.path.dirname(torch.__file__)
+    host = [[os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + os.path.join(t, "include"),
+             "-I" + sysconfig.get_paths()["include"], "-I/opt/rocm/include", bind, "-o", HOST, "-L" + os.path.join(t, "lib"),
+             "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]]
+
   with ThreadPoolExecutor(max_workers=4) as ex:
-    list(ex.map(run, jobs))
+    list(ex.map(run, host + jobs))
   if jobs or _stale(OUT, objs):
     run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", OUT] + objs)
   return OUT

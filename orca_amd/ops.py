@@ -1,10 +1,7 @@
 """Torch-tensor front end of the C ABI (include/orca_hip.h).  torch is used for device memory and
 streams only; every function below is one call into liborca_hip.so on the current HIP stream.
 There is no CPU fallback: tensors must live on a HIP device and the library must be built."""
-import array
 import ctypes
-import itertools
-import operator
 from typing import NamedTuple
 
 import numpy as np
@@ -587,109 +584,8 @@ def decoder_train(emb, fc1_w, fc1_b, fc2_w, fc2_b, want_prob=False, pool=None):
 
 # ---------------------------------------------------------------------------------------------
 # embedding tables with gradients; gradient norm and clipping
+# (csrc/bind.cpp checks the tensors, allocates and calls the C ABI on the current stream of the tensors' device)
 # ---------------------------------------------------------------------------------------------
-_ELEM = {torch.float32: _lib.ORCA_F32, torch.bfloat16: _lib.ORCA_BF16, torch.float16: _lib.ORCA_F16}
-
-
-def _elem(t, what):
-  code = _ELEM.get(t.dtype) if isinstance(t, torch.Tensor) else None
-  if code is None:
-    raise TypeError(f"{what}: expected a float32, bfloat16 or float16 tensor, got {getattr(t, 'dtype', type(t))}")
-  if not t.is_cuda:
-    raise _lib.OrcaError(f"{what}: expected a tensor on the HIP device (no CPU fallback)")
-  return code
-
-
-def _id_list(ids, dev, what):
-  """ids flattened without a copy where they can be, and their address as (int64 list, int32 list)"""
-  if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int64, torch.int32):
-    raise TypeError(f"{what}: ids must be an int64 or int32 tensor, got {getattr(ids, 'dtype', type(ids))}")
-  if ids.device != dev:
-    raise _lib.OrcaError(f"{what}: ids are on {ids.device}, the rows on {dev}")
-  ids = ids.contiguous()
-  return (ids, ids.data_ptr(), None) if ids.dtype is torch.int64 else (ids, None, ids.data_ptr())
-
-
-def _row_view(t, width, what):
-  """t as rows of `width` elements that lie one element apart: itself (any row stride, 0 included), or a copy"""
-  t = t.reshape(-1, width)
-  return t if t.stride(1) == 1 or width == 1 else t.contiguous()
-
-
-def _on(device):
-  """calls for tensors of another device than the current one go to that device's current stream"""
-  return torch.cuda.device(device)
-
-
-def embedding(table, ids, scale=1.0, out=None):
-  """orca_embedding_forward: scale * table[ids] -- table [n_rows, width] fp32 / bf16 / fp16 (rows may be strided), ids int64 or
-  int32 of any shape -> [*ids.shape, width] in the table's type (fp32 product, one rounding).  An id outside the table reads as
-  zeros.  out: a contiguous tensor of that shape and type.  No autograd: torch.ops.orca.embedding has it."""
-  code = _elem(table, "embedding table")
-  dev = table.device
-  if table.dim() != 2:
-    raise ValueError(f"embedding: table has shape {tuple(table.shape)}, expected [n_rows, width]")
-  if dev.index != torch.cuda.current_device():
-    with _on(dev):
-      return embedding(table, ids, scale, out)
-  ids, i64, i32 = _id_list(ids, dev, "embedding")
-  n_rows, width = table.shape
-  if width != 1 and table.stride(1) != 1:
-    raise ValueError(f"embedding: the table's columns lie {table.stride(1)} elements apart (a copy of a table is the caller's to make)")
-  shape = (*ids.shape, width)
-  if out is None:
-    out = torch.empty(shape, dtype=table.dtype, device=dev)
-  elif out.shape != shape or out.dtype != table.dtype or out.device != dev or not out.is_contiguous():
-    raise ValueError(f"embedding: out must be a contiguous {table.dtype} tensor of shape {shape} on {dev}")
-  check(_lib.load().orca_embedding_forward(table.data_ptr(), code, n_rows, width, table.stride(0), i64, i32, ids.numel(), scale,
-                                           out.data_ptr(), stream()), "orca_embedding_forward")
-  return out
-
-
-def _backward_args(who, grad_out, ids, num_rows, dtype):
-  """what both forms of the gradient check: (gradient rows, ids, address pair, type codes, device, workspace)"""
-  code = _elem(grad_out, f"{who} grad_out")
-  dev = grad_out.device
-  ids, i64, i32 = _id_list(ids, dev, who)
-  if grad_out.dim() < 1 or grad_out.shape[:-1] != ids.shape:
-    raise ValueError(f"{who}: grad_out has shape {tuple(grad_out.shape)}, expected {tuple(ids.shape)} + (width,)")
-  dtype = grad_out.dtype if dtype is None else dtype
-  if dtype not in (grad_out.dtype, torch.float32):
-    raise TypeError(f"{who}: a {grad_out.dtype} gradient cannot be returned as {dtype} (its own type, or float32)")
-  width = grad_out.shape[-1]
-  n = ids.numel()
-  g = _row_view(grad_out, width, who) if n and width else grad_out
-  nbytes = _lib.load().orca_embedding_backward_workspace_bytes(n, width, int(num_rows))
-  if nbytes < 0:
-    raise ValueError(f"{who}: unsupported sizes: {n} ids, width {width}, {num_rows} rows")
-  return g, ids, i64, i32, n, width, code, dtype, dev, torch.empty(nbytes, dtype=torch.uint8, device=dev), nbytes
-
-
-def embedding_backward(grad_out, ids, num_rows, scale=1.0, padding_idx=None, out=None, accumulate=False, dtype=None):
-  """orca_embedding_backward: the gradient of embedding() for its table as a dense [num_rows, width] tensor: row v is scale * the
-  sum of grad_out over the places where ids is v (fp32 sums in a fixed order: the same call gives the same bits).  Ids outside
-  [0, num_rows) and padding_idx (None or negative: no such id) contribute nothing.  dtype: grad_out's (the default) or float32.
-  out: a [num_rows, width] tensor of that type (rows may be strided, not overlapping); accumulate adds into it."""
-  if isinstance(grad_out, torch.Tensor) and grad_out.is_cuda and grad_out.device.index != torch.cuda.current_device():
-    with _on(grad_out.device):
-      return embedding_backward(grad_out, ids, num_rows, scale, padding_idx, out, accumulate, dtype)
-  if out is not None and dtype is None and isinstance(out, torch.Tensor):
-    dtype = out.dtype
-  g, ids, i64, i32, n, width, code, dtype, dev, ws, nbytes = _backward_args("embedding_backward", grad_out, ids, num_rows, dtype)
-  shape = (int(num_rows), width)
-  if out is None:
-    if accumulate:
-      raise ValueError("embedding_backward: accumulate needs out")
-    out = torch.empty(shape, dtype=dtype, device=dev)
-  elif out.shape != shape or out.dtype != dtype or out.device != dev or (width > 1 and out.stride(1) != 1) or \
-      (shape[0] > 1 and out.stride(0) < width):
-    raise ValueError(f"embedding_backward: out must be a {dtype} tensor of shape {shape} on {dev} whose rows are contiguous and do not overlap")
-  check(_lib.load().orca_embedding_backward(g.data_ptr() if n else None, code, g.stride(0) if n else 0, i64, i32, n, width, shape[0],
-                                            -1 if padding_idx is None else int(padding_idx), scale, 1 if accumulate else 0, out.data_ptr(),
-                                            _ELEM[dtype], out.stride(0), ws.data_ptr(), nbytes, stream()), "orca_embedding_backward")
-  return out
-
-
 class RowGrad(NamedTuple):
   """A row-sparse gradient of a [num_rows, width] table: rows[r] is the gradient of row ids[r] for r < count (a device int); what
   lies behind is unused.  ids are distinct and ascend."""
@@ -699,121 +595,60 @@ class RowGrad(NamedTuple):
   num_rows: int
 
 
+_host = None
+
+
+def _load_host():
+  global _host
+  lib = _lib.load()
+  try:
+    from . import _host as h
+  except ImportError as e:
+    raise _lib.OrcaError(f"orca_amd/_host.so is missing or does not load ({e}): build it with `python -m orca_amd.build`") from e
+  h.setup(_lib.OrcaError, RowGrad, *(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
+      "orca_last_error", "orca_embedding_forward", "orca_embedding_backward_workspace_bytes", "orca_embedding_backward",
+      "orca_embedding_backward_rows", "orca_grad_norm_workspace_bytes", "orca_grad_norm", "orca_clip_grads")))
+  _host = h
+  return h
+
+
+def embedding(table, ids, scale=1.0, out=None):
+  """orca_embedding_forward: scale * table[ids] -- table [n_rows, width] fp32 / bf16 / fp16 (rows may be strided), ids int64 or
+  int32 of any shape -> [*ids.shape, width] in the table's type (fp32 product, one rounding).  An id outside the table reads as
+  zeros.  out: a contiguous tensor of that shape and type.  No autograd: torch.ops.orca.embedding has it."""
+  return (_host or _load_host()).embedding(table, ids, scale, out)
+
+
+def embedding_backward(grad_out, ids, num_rows, scale=1.0, padding_idx=None, out=None, accumulate=False, dtype=None):
+  """orca_embedding_backward: the gradient of embedding() for its table as a dense [num_rows, width] tensor: row v is scale * the
+  sum of grad_out over the places where ids is v (fp32 sums in a fixed order: the same call gives the same bits).  Ids outside
+  [0, num_rows) and padding_idx (None or negative: no such id) contribute nothing.  dtype: grad_out's (the default) or float32.
+  out: a [num_rows, width] tensor of one of those types (rows may be strided, not overlapping); accumulate adds into it."""
+  return (_host or _load_host()).embedding_backward(grad_out, ids, num_rows, scale, padding_idx, out, accumulate, dtype)
+
+
 def embedding_backward_rows(grad_out, ids, num_rows, scale=1.0, padding_idx=None, out=None, dtype=None):
   """orca_embedding_backward_rows: embedding_backward's rows that an id contributes to, as a RowGrad with room for ids.numel() rows.
   out: (ids int64 [n], rows [n, width], count int32 [1]) or a RowGrad to fill, contiguous; what lies behind its last row is left
   as it was.  No host read: the count stays on the device."""
-  if isinstance(grad_out, torch.Tensor) and grad_out.is_cuda and grad_out.device.index != torch.cuda.current_device():
-    with _on(grad_out.device):
-      return embedding_backward_rows(grad_out, ids, num_rows, scale, padding_idx, out, dtype)
-  if out is not None and dtype is None:
-    dtype = out[1].dtype
-  g, ids, i64, i32, n, width, code, dtype, dev, ws, nbytes = _backward_args("embedding_backward_rows", grad_out, ids, num_rows, dtype)
-  if out is None:
-    r_ids = torch.empty(n, dtype=torch.int64, device=dev)
-    rows = torch.empty((n, width), dtype=dtype, device=dev)
-    count = torch.empty(1, dtype=torch.int32, device=dev)
-  else:
-    r_ids, rows, count = out[:3]
-    if r_ids.shape != (n,) or r_ids.dtype != torch.int64 or rows.shape != (n, width) or rows.dtype != dtype or count.shape != (1,) or \
-        count.dtype != torch.int32 or not (r_ids.device == rows.device == count.device == dev) or \
-        not (r_ids.is_contiguous() and rows.is_contiguous()):
-      raise ValueError(f"embedding_backward_rows: out must be contiguous int64 [{n}], {dtype} [{n}, {width}] and int32 [1] tensors on {dev}")
-  check(_lib.load().orca_embedding_backward_rows(g.data_ptr() if n else None, code, g.stride(0) if n else 0, i64, i32, n, width, int(num_rows),
-                                                 -1 if padding_idx is None else int(padding_idx), scale, r_ids.data_ptr(), rows.data_ptr(),
-                                                 _ELEM[dtype], count.data_ptr(), ws.data_ptr(), nbytes, stream()),
-        "orca_embedding_backward_rows")
-  return RowGrad(r_ids, rows, count, int(num_rows))
-
-
-_GETDTYPE = operator.attrgetter("dtype")
-_TENSOR = torch.Tensor
-_NORM_WORK = 16384     # orca_grad_norm_workspace_bytes()
-
-
-def _grad_list(who, grads):
-  """a list (or the values of a dict) of tensors and RowGrads as the host arrays of orca_grad_norm / orca_clip_grads.  Returns (n,
-  arrays, device, tensors, copies): tensors[i] is what array i points to, copies = the places that hold a contiguous copy."""
-  grads = [g for g in (grads.values() if isinstance(grads, dict) else grads) if g is not None]
-  rows = widths = None
-  if RowGrad in set(map(type, grads)):
-    rows = array.array("Q", [g.count.data_ptr() if type(g) is RowGrad else 0 for g in grads])
-    widths = array.array("i", [g.rows.shape[1] if type(g) is RowGrad else 0 for g in grads])
-    grads = [g.rows if type(g) is RowGrad else g for g in grads]
-  try:
-    kinds = bytes(map(_ELEM.__getitem__, map(_GETDTYPE, grads)))
-  except (KeyError, AttributeError):
-    raise TypeError(f"{who}: gradients must be float32, bfloat16 or float16 tensors") from None
-  where = set(map(_TENSOR.get_device, grads))
-  if len(where) > 1 or -1 in where:
-    raise _lib.OrcaError(f"{who}: the gradients must be on one HIP device (no CPU fallback)")
-  copies = []
-  if not all(map(_TENSOR.is_contiguous, grads)):
-    for i, g in enumerate(grads):
-      if not g.is_contiguous():
-        copies.append((i, g))
-        grads[i] = g.contiguous()
-  return grads, kinds, rows, widths, (where.pop() if where else torch.cuda.current_device()), copies
-
-
-def _address(a):
-  return a.buffer_info()[0] if a is not None else None
+  return RowGrad(*(_host or _load_host()).embedding_backward_rows(grad_out, ids, num_rows, scale, padding_idx, out, dtype), num_rows)
 
 
 def grad_norm(grads, max_norm=None):
   """orca_grad_norm: the 2-norm over all tensors of a list (or a dict's values; None entries are left out) of fp32 / bf16 / fp16
   tensors and RowGrads, squares and sums in fp64, as a float32 scalar tensor on the device.  max_norm: also returns min(1, max_norm /
-  (norm + 1e-6)) as a scalar tensor -- what FusedAdam.step takes as grad_scale."""
-  ts, kinds, rows, widths, dev, _ = _grad_list("grad_norm", grads)
-  if dev != torch.cuda.current_device():
-    with _on(dev):
-      return grad_norm(grads, max_norm)
-  device = torch.device("cuda", dev)
-  norm, coef = torch.empty((), dtype=torch.float32, device=device), torch.empty((), dtype=torch.float32, device=device)
-  ws = torch.empty(_NORM_WORK, dtype=torch.uint8, device=device)
-  ptrs, sizes = array.array("Q", map(_TENSOR.data_ptr, ts)), array.array("q", map(_TENSOR.numel, ts))
-  check(_lib.load().orca_grad_norm(len(ts), _address(ptrs), _address(sizes), kinds, _address(rows), _address(widths),
-                                   0.0 if max_norm is None else max_norm, norm.data_ptr(), coef.data_ptr(), ws.data_ptr(), stream()),
-        "orca_grad_norm")
-  return norm if max_norm is None else (norm, coef)
+  (norm + 1e-6)) as a scalar tensor."""
+  return (_host or _load_host()).grad_norm(list(grads.values() if isinstance(grads, dict) else grads), max_norm)
 
 
 def clip_grad_norm(grads, max_norm, flat=None):
   """orca_clip_grads: grad_norm(grads), and every gradient scaled by min(1, max_norm / (norm + 1e-6)) as torch.nn.utils.clip_grad_norm_
   does (product in fp32, one rounding; a norm that is not finite makes the gradients NaN or 0 as there).  In place, or with flat = a
-  contiguous 1-D tensor for each type among the gradients (in the order in which the types first appear), where the products of that
+  contiguous tensor for each type among the gradients (in the order in which the types first appear), where the products of that
   type's gradients go one after another and the gradients stay as they are.  Returns the norm before clipping as a float32 scalar
   tensor; nothing is read by the host."""
-  ts, kinds, rows, widths, dev, copies = _grad_list("clip_grad_norm", grads)
-  if dev != torch.cuda.current_device():
-    with _on(dev):
-      return clip_grad_norm(grads, max_norm, flat)
-  ptrs, sizes = array.array("Q", map(_TENSOR.data_ptr, ts)), array.array("q", map(_TENSOR.numel, ts))
-  bufs = None
-  if flat is None:
-    if len(set(ptrs)) != len(ptrs) and len(set(p for p, s in zip(ptrs, sizes) if s)) != sum(1 for s in sizes if s):
-      raise ValueError("clip_grad_norm: a gradient is in the list twice")
-    for _, g in copies:
-      if any(st == 0 and sz > 1 for st, sz in zip(g.stride(), g.shape)):
-        raise ValueError("clip_grad_norm: an expanded tensor cannot be clipped in place")
-  else:
-    bufs = array.array("Q", (0, 0, 0))
-    order = list(dict.fromkeys(kinds))
-    if len(flat) != len(order):
-      raise ValueError(f"clip_grad_norm: {len(flat)} flat buffers for gradients of {len(order)} types")
-    for code, f in zip(order, flat):
-      need = sum(sizes) if len(order) == 1 else sum(itertools.compress(sizes, map(code.__eq__, kinds)))
-      if _elem(f, "clip_grad_norm flat") != code or f.numel() != need or f.get_device() != dev or not f.is_contiguous():
-        raise ValueError(f"clip_grad_norm: a flat buffer is not a contiguous tensor of {need} elements of its gradients' type and device")
-      bufs[code] = f.data_ptr()
-  device = torch.device("cuda", dev)
-  norm, ws = torch.empty((), dtype=torch.float32, device=device), torch.empty(_NORM_WORK, dtype=torch.uint8, device=device)
-  check(_lib.load().orca_clip_grads(len(ts), _address(ptrs), _address(sizes), kinds, _address(rows), _address(widths), max_norm, _address(bufs),
-                                    norm.data_ptr(), ws.data_ptr(), stream()), "orca_clip_grads")
-  if flat is None:
-    for i, g in copies:
-      g.copy_(ts[i])
-  return norm
+  return (_host or _load_host()).clip_grad_norm(list(grads.values() if isinstance(grads, dict) else grads), max_norm,
+                                                None if flat is None else list(flat))
 
 
 class FusedAdam:
