@@ -99,7 +99,7 @@ __device__ __forceinline__ void scale(const u32x4 (&r)[STEPS], const piece& q, c
       unpack16<T>(r[k], f);
 #pragma unroll
       for (int j = 0; j < elems16<T>; ++j) f[j] *= c;
-      if constexpr (STREAMS) __builtin_nontemporal_store(pack16<T>(f), reinterpret_cast<u32x4_any*>(out + b));
+      if constexpr (STREAMS) store16_past(out + b, pack16<T>(f));
       else store16(out + b, pack16<T>(f));
     } else {
       for (int e = b; e < q.len; e += (int)sizeof(T))
@@ -113,7 +113,7 @@ __device__ __forceinline__ void request(u32x4 (&r)[STEPS], const piece& q) {
   for (int k = 0; k < STEPS; ++k) {
     const int b = ((int)threadIdx.x + 256 * k) * 16;
     if (b + 16 <= q.len) {
-      if constexpr (STREAMS) r[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(q.p + q.offset + b));
+      if constexpr (STREAMS) r[k] = load16_past(q.p + q.offset + b);
       else r[k] = load16(q.p + q.offset + b);
     }
   }

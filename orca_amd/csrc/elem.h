@@ -11,6 +11,10 @@ template <class T> constexpr int elems16 = 16 / (int)sizeof(T);
 
 __device__ __forceinline__ u32x4 load16(const void* p) { return *reinterpret_cast<const u32x4_any*>(p); }
 __device__ __forceinline__ void store16(void* p, u32x4 v) { *reinterpret_cast<u32x4_any*>(p) = v; }
+// the same past the caches (non-temporal).  The choice has to be a template's: the compiler merges the two sides of a branch on a
+// run-time flag into one plain access.
+__device__ __forceinline__ u32x4 load16_past(const void* p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p)); }
+__device__ __forceinline__ void store16_past(void* p, u32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p)); }
 
 template <class T> __device__ __forceinline__ void unpack16(u32x4 r, float (&f)[elems16<T>]) {
   T e[elems16<T>];

@@ -14,15 +14,28 @@ template <int VEC, class T> __device__ __forceinline__ void load_chunk(const T* 
   if constexpr (VEC == 1) f[0] = (float)p[0];
   else unpack16<T>(load16(p), f);
 }
-template <int VEC, class T> __device__ __forceinline__ void store_chunk(T* p, const float (&f)[VEC]) {
+template <int VEC, class T, bool PAST = false> __device__ __forceinline__ void store_chunk(T* p, const float (&f)[VEC]) {
   if constexpr (VEC * sizeof(T) < 16) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) p[j] = (T)f[j];
   } else {
 #pragma unroll
-    for (int k = 0; k < VEC; k += elems16<T>) store16(p + k, pack16<T>(f + k));
+    for (int k = 0; k < VEC; k += elems16<T>) {
+      if constexpr (PAST) store16_past(p + k, pack16<T>(f + k));
+      else store16(p + k, pack16<T>(f + k));
+    }
   }
 }
+
+// Where accesses go past the caches, by the bytes they cover.  Measured with the pass that reads or writes them next to it (us, plain
+// -> past): lookup and a product over its output 17 MB 14.0 -> 13.3, 21 MB 16.0 -> 16.4, 128 MB 85 -> 94, 256 MB 192 -> 193, 512 MB
+// 372 -> 359 (the lookup alone 7.3 -> 5.6, .., 178 -> 149); dense gradient and the norm of it 256 MB 104 -> 112, 400 MB 164 -> 162,
+// 800 MB 318 -> 302; a product over grad_out and the gradient's pass over it 96 MB 70 -> 73, 128 MB 86.5 -> 85.8, 256 MB 156 -> 147.
+// In between, the 256 MB last-level cache hands the bytes to the neighbour.
+constexpr int64_t MB = 1000000;
+bool past_lookup(int64_t bytes) { return bytes <= 19 * MB || bytes >= 256 * MB; }
+bool past_zeros(int64_t bytes) { return bytes >= 384 * MB; }
+bool past_gradient(int64_t bytes) { return bytes >= 128 * MB; }
 
 constexpr int64_t MAX_WIDTH = 65536;      // x * C of the division below stays under 2^32
 
@@ -30,7 +43,7 @@ constexpr int64_t MAX_WIDTH = 65536;      // x * C of the division below stays u
 // The output is a list of n * C chunks of 16 bytes; the last chunk of a row starts at width - VEC, so that every access is
 // whole (it overlaps the one before it: both write the same values).  Rows narrower than a chunk go element by element.
 constexpr int LOOK_U = 4;                 // chunks per thread: that many independent id -> row chains
-template <class T, int VEC, class I>
+template <class T, int VEC, bool PAST, class I>
 __global__ __launch_bounds__(256) void k_embedding(const T* __restrict__ table, int64_t n_rows, int64_t ld,
                                                    const I* __restrict__ ids, int64_t total, int width, uint32_t C,
                                                    uint32_t magic, float scale, T* __restrict__ out) {
@@ -66,7 +79,7 @@ __global__ __launch_bounds__(256) void k_embedding(const T* __restrict__ table, 
     if (row[u] >= 0 && row[u] < n_rows)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[u][j] *= scale;
-    store_chunk<VEC, T>(out + at[u], v[u]);
+    store_chunk<VEC, T, PAST>(out + at[u], v[u]);
   }
 }
 
@@ -76,8 +89,8 @@ int launch_embedding(const void* table, int64_t n_rows, int64_t width, int64_t l
   const int64_t C = ceil_div64(width, VEC), total = n * C, blocks = ceil_div64(total, 256 * LOOK_U);
   ORCA_REQUIRE(blocks < (1LL << 31), "orca_embedding_forward: %lld rows of %lld values are too many for one call", (long long)n, (long long)width);
   const uint32_t magic = C == 1 ? 0 : (uint32_t)(((1ULL << 32) + C - 1) / C);
-  k_embedding<T, VEC, I><<<(unsigned)blocks, 256, 0, stream>>>((const T*)table, n_rows, ld, ids, total, (int)width, (uint32_t)C, magic, scale,
-                                                               (T*)out);
+  auto* kernel = VEC > 1 && past_lookup(n * width * (int64_t)sizeof(T)) ? k_embedding<T, VEC, VEC != 1, I> : k_embedding<T, VEC, false, I>;
+  kernel<<<(unsigned)blocks, 256, 0, stream>>>((const T*)table, n_rows, ld, ids, total, (int)width, (uint32_t)C, magic, scale, (T*)out);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
@@ -100,8 +113,9 @@ constexpr int FILL_PIECE = 32768;       // bytes a workgroup writes at a time
 struct fill_job {
   char* p;                      // `rows` rows of `bytes` bytes, `pitch` bytes apart (a table without gaps is one row)
   int64_t bytes, pitch, per_row, from, to;      // pieces of a row; this launch's pieces
+  int past;
 };
-template <int THREADS> __device__ __forceinline__ void fill_pieces(const fill_job& f, int64_t block, int64_t blocks) {
+template <int THREADS, bool PAST> __device__ __forceinline__ void fill_loop(const fill_job& f, int64_t block, int64_t blocks) {
   const u32x4 zero = {0, 0, 0, 0};
   for (int64_t i = f.from + block; i < f.to; i += blocks) {
     const int64_t r = i / f.per_row, at = (i - r * f.per_row) * FILL_PIECE;
@@ -111,12 +125,17 @@ template <int THREADS> __device__ __forceinline__ void fill_pieces(const fill_jo
     for (int k = 0; k < FILL_PIECE / (16 * THREADS); ++k) {
       const int b = ((int)threadIdx.x + THREADS * k) * 16;
       if (b + 16 <= len) {
-        store16(p + b, zero);
+        if constexpr (PAST) store16_past(p + b, zero);
+        else store16(p + b, zero);
       } else {
         for (int e = b; e < len; e += 2) *reinterpret_cast<uint16_t*>(p + e) = 0;
       }
     }
   }
+}
+template <int THREADS> __device__ __forceinline__ void fill_pieces(const fill_job& f, int64_t block, int64_t blocks) {
+  if (f.past) fill_loop<THREADS, true>(f, block, blocks);
+  else fill_loop<THREADS, false>(f, block, blocks);
 }
 __global__ __launch_bounds__(512) void k_fill(fill_job f) { fill_pieces<512>(f, blockIdx.x, gridDim.x); }
 
@@ -377,7 +396,10 @@ struct seg_args {
 
 template <int VEC, class T> struct raw_chunk {        // a chunk as it was loaded
   u32x4 r;
-  __device__ __forceinline__ void load(const T* p) { r = load16(p); }
+  template <bool PAST = false> __device__ __forceinline__ void load(const T* p) {
+    if constexpr (PAST) r = load16_past(p);
+    else r = load16(p);
+  }
   __device__ __forceinline__ void add_to(float (&acc)[VEC]) const {
     float f[VEC];
     unpack16<T>(r, f);
@@ -387,11 +409,11 @@ template <int VEC, class T> struct raw_chunk {        // a chunk as it was loade
 };
 template <class T> struct raw_chunk<1, T> {
   T r;
-  __device__ __forceinline__ void load(const T* p) { r = *p; }
+  template <bool PAST = false> __device__ __forceinline__ void load(const T* p) { r = *p; }
   __device__ __forceinline__ void add_to(float (&acc)[1]) const { acc[0] += (float)r; }
 };
 
-template <class TI, class TO, int VEC, bool ACCUMULATE>
+template <class TI, class TO, int VEC, bool ACCUMULATE, bool PAST>
 __global__ __launch_bounds__(256) void k_segment_sum(seg_args a) {
   __shared__ pair32 list[SEG_PAIRS + 2];        // [k + 1] = pair k of the workgroup's windows; its neighbours at both ends
   __shared__ uint32_t row[SEG_PAIRS];           // [k] = the output row of pair k (row-sparse form)
@@ -440,7 +462,7 @@ __global__ __launch_bounds__(256) void k_segment_sum(seg_args a) {
   typedef raw_chunk<VEC, TI> raw;
   auto request = [&](raw (&v)[SEG_U], int k) {
 #pragma unroll
-    for (int u = 0; u < SEG_U; ++u) v[u].load(g + (int64_t)list[min(k + u, last - 1) + 1].pos * a.ld_g);
+    for (int u = 0; u < SEG_U; ++u) v[u].template load<PAST>(g + (int64_t)list[min(k + u, last - 1) + 1].pos * a.ld_g);
   };
   auto add = [&](const raw (&v)[SEG_U], int k) {
 #pragma unroll
@@ -1045,8 +1067,10 @@ int launch_sums_vec(seg_args a, bool accumulate, hipStream_t stream) {
   a.col_blocks = (int)ceil_div64(a.chunks, 1 << a.log_l);
   const int64_t windows = ceil_div64(a.n, a.window), blocks = ceil_div64(windows, 256 >> a.log_l) * a.col_blocks;
   ORCA_REQUIRE(blocks < (1LL << 31), "orca_embedding_backward: %lld ids of width %d are too many for one call", (long long)a.n, a.width);
-  if (accumulate) k_segment_sum<TI, TO, VEC, true><<<(unsigned)blocks, 256, 0, stream>>>(a);
-  else k_segment_sum<TI, TO, VEC, false><<<(unsigned)blocks, 256, 0, stream>>>(a);
+  const bool past = VEC > 1 && past_gradient(a.n * a.width * (int64_t)sizeof(TI));
+  auto* kernel = accumulate ? (past ? k_segment_sum<TI, TO, VEC, true, VEC != 1> : k_segment_sum<TI, TO, VEC, true, false>)
+                            : (past ? k_segment_sum<TI, TO, VEC, false, VEC != 1> : k_segment_sum<TI, TO, VEC, false, false>);
+  kernel<<<(unsigned)blocks, 256, 0, stream>>>(a);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
@@ -1241,6 +1265,7 @@ ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64
     fill.pitch = ld_table * e;
     fill.per_row = ceil_div64(fill.bytes, FILL_PIECE);
     pieces = (gaps ? num_rows : 1) * fill.per_row;
+    fill.past = past_zeros(num_rows * width * e);
   }
   if (n == 0) {
     if (pieces) k_fill<<<fill_share(&fill, pieces, 0, 1), 512, 0, stream>>>(fill);
