@@ -148,6 +148,7 @@ constexpr int SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_ITEMS = 4
 constexpr int MIN_DIGIT = 2, MAX_DIGIT = 11, MAX_BINS = 1 << MAX_DIGIT;
 constexpr int DIRECT_TILES = 64;        // up to this many tiles every workgroup adds the counts up itself
 static_assert(SORT_TILE <= 65536, "16-bit counts within a tile");
+static_assert(2 * SORT_THREADS * 16 <= SORT_WAVES * MAX_BINS * 2, "the slices' sums fit where the counts lie");
 static_assert(MAX_BINS == 4 * SORT_THREADS, "a thread takes four neighbouring bins");
 struct pair32 { uint32_t pos, key; };
 
@@ -247,25 +248,39 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
     const int64_t i = base + 64 * u + lane;
     p[u] = i < src.n ? sort_read(src, i) : pair32{0u, 0u};
   }
-  // the thread's four bins: pairs of them in the tiles before this one, and in all
+  // pairs of each bin in the tiles before this one, and in all: a thread takes four bins and every `slices`-th tile
   u32x4 before = {0, 0, 0, 0}, total = {0, 0, 0, 0};
-  if (4 * t < bins) {
-    if (totals) {
-      before = load16(counts + (int64_t)blockIdx.x * bins + 4 * t);
-      total = load16(totals + 4 * t);
-    } else {
-      for (int k0 = 0; k0 < tiles; k0 += 8) {
-        u32x4 c[8];
+  const int quads = bins / 4, slices = SORT_THREADS / quads, quad = t & (quads - 1), slice = t / quads;
+  if (totals) {
+    if (slice == 0) {
+      before = load16(counts + (int64_t)blockIdx.x * bins + 4 * quad);
+      total = load16(totals + 4 * quad);
+    }
+  } else {
+    for (int k0 = slice; k0 < tiles; k0 += 8 * slices) {
+      u32x4 c[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) c[u] = k0 + u < tiles ? load16(counts + (int64_t)(k0 + u) * bins + 4 * t) : u32x4{0, 0, 0, 0};
+      for (int u = 0; u < 8; ++u) c[u] = k0 + u * slices < tiles ? load16(counts + (int64_t)(k0 + u * slices) * bins + 4 * quad) : u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (k0 + u < (int)blockIdx.x) before += c[u];
-          total += c[u];
-        }
+      for (int u = 0; u < 8; ++u) {
+        if (k0 + u * slices < (int)blockIdx.x) before += c[u];
+        total += c[u];
       }
     }
+    if (slices > 1) {           // the slices' sums meet in LDS (`part` is not in use yet)
+      u32x4* meet = reinterpret_cast<u32x4*>(&part[0][0]);
+      meet[t] = before;
+      meet[SORT_THREADS + t] = total;
+      __syncthreads();
+      if (slice == 0)
+        for (int k = 1; k < slices; ++k) {
+          before += meet[quad + k * quads];
+          total += meet[SORT_THREADS + quad + k * quads];
+        }
+      __syncthreads();
+    }
   }
+  if (slice != 0) total = u32x4{0, 0, 0, 0};
   for (int k = t; k < SORT_WAVES * MAX_BINS / 8; k += SORT_THREADS) reinterpret_cast<u32x4*>(&part[0][0])[k] = u32x4{0, 0, 0, 0};
   __syncthreads();
   uint32_t rank[SORT_ITEMS];
@@ -288,8 +303,9 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
   if (lane == 63) wave_sum[wave] = inc;
   __syncthreads();
   uint32_t run = inc - mine;
-  for (int w = 0; w < wave; ++w) run += wave_sum[w];
-  if (4 * t < bins) {
+#pragma unroll
+  for (int w = 0; w < SORT_WAVES; ++w) run += w < wave ? wave_sum[w] : 0u;
+  if (slice == 0) {             // (t == quad)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int b = 4 * t + k;
@@ -424,10 +440,11 @@ __global__ __launch_bounds__(256) void k_segment_sum(seg_args a) {
   const int count = (int)(a.n - base < teams * a.window ? a.n - base : teams * a.window);
   for (int k = threadIdx.x; k < count + 2; k += 256) {
     const int64_t i = base - 1 + k;
-    list[k] = i >= 0 && i < a.n ? a.s[i] : pair32{0u, ~0u};          // (~0u: no key)
+    const pair32 p = i >= 0 && i < a.n ? a.s[i] : pair32{0u, ~0u};          // (~0u: no key)
+    const uint32_t r = a.rank && k < count ? a.rank[base + k] : 0u;          // (here: in the loop below it would wait for the rows on their way)
+    list[k] = p;
+    if (k < count) row[k] = r;
   }
-  if (a.rank)       // (ahead of the loop: a load inside it would wait for the rows on their way)
-    for (int k = threadIdx.x; k < count; k += 256) row[k] = a.rank[base + k];
   __syncthreads();
   const int first = team * a.window, last = min(first + a.window, count);
   if (first >= count || c >= a.chunks || list[first + 1].key == a.none) return;
@@ -495,13 +512,14 @@ __global__ __launch_bounds__(256) void k_segment_sum(seg_args a) {
 // The runs that cross window borders, each taken by the window that begins it: sum of what that window and the following ones left in
 // `part`, in their order.  A team takes one window; a run over more than JOIN_SHORT windows is left to the whole workgroup, whose teams
 // take a consecutive share of the terms each.
-constexpr int JOIN_SHORT = 16;
+constexpr int JOIN_SHORT = 16, JOIN_THREADS = 1024;
 template <class TO, bool ACCUMULATE>
-__global__ __launch_bounds__(256) void k_segment_join(seg_args a) {
-  __shared__ float4 share[256];
-  __shared__ int64_t queue[256];
+__global__ __launch_bounds__(JOIN_THREADS) void k_segment_join(seg_args a) {
+  __shared__ float4 share[JOIN_THREADS];
+  struct waiting { int64_t w, r; uint32_t key; };
+  __shared__ waiting queue[JOIN_THREADS];
   __shared__ int queued;
-  const int lanes = 1 << a.log_l, teams = 256 >> a.log_l, team = threadIdx.x >> a.log_l, tl = threadIdx.x & (lanes - 1);
+  const int lanes = 1 << a.log_l, teams = JOIN_THREADS >> a.log_l, team = threadIdx.x >> a.log_l, tl = threadIdx.x & (lanes - 1);
   const int64_t w = (int64_t)(blockIdx.x / (uint32_t)a.col_blocks) * teams + team;
   const int col = (((int)(blockIdx.x % (uint32_t)a.col_blocks) << a.log_l) + tl) * 4;
   const int have = col >= a.width ? 0 : min(4, a.width - col);
@@ -531,43 +549,46 @@ __global__ __launch_bounds__(256) void k_segment_join(seg_args a) {
     }
     return acc;
   };
-  auto write = [&](int64_t w, uint32_t key, float4 acc) {
-    const int64_t r = a.rank ? (int64_t)a.rank[(w + 1) * a.window - 1] : (int64_t)key;
+  auto write = [&](int64_t r, float4 acc) {
     TO* o = (TO*)a.out + r * a.ld_out + col;
     const float f[4] = {acc.x * a.scale, acc.y * a.scale, acc.z * a.scale, acc.w * a.scale};
     for (int j = 0; j < have; ++j) o[j] = (TO)(ACCUMULATE ? (float)o[j] + f[j] : f[j]);
   };
-  const int64_t i0 = w * a.window, i1 = i0 + a.window;
-  if (i1 < a.n) {
-    const uint32_t key = a.s[i1 - 1].key;
-    if (key != a.none && a.s[i1].key == key && !(i0 > 0 && a.s[i0 - 1].key == key)) {       // (the same in the team's lanes)
-      int terms = 1;
-      for (int t0 = 1; t0 <= JOIN_SHORT; t0 += lanes) {
-        const int64_t f = (w + t0 + tl) * a.window;
-        const uint64_t m = __ballot(f < a.n && a.s[f].key == key);
-        const uint64_t of_team = lanes == 64 ? m : (m >> (threadIdx.x & 63 & ~(lanes - 1))) & ((1ULL << lanes) - 1);
-        const int in = __popcll(of_team);
-        terms += in;
-        if (in < lanes) break;
-      }
-      if (terms <= JOIN_SHORT) {
-        write(w, key, sum(w, 0, terms));
-      } else if (tl == 0) {
-        queue[atomicAdd(&queued, 1)] = w;
-      }
+  // what decides about the window, requested together: a run costs two round trips (this one, its terms), not one per question
+  const int64_t i0 = w * a.window, i1 = i0 + a.window, end = a.n - 1;
+  const uint32_t key = a.s[i1 - 1 < end ? i1 - 1 : end].key, next = a.s[i1 < end ? i1 : end].key, prev = a.s[i0 > 0 && i0 <= end ? i0 - 1 : 0].key;
+  const int64_t f0 = (w + 1 + tl) * a.window;
+  const uint32_t later = a.s[f0 < end ? f0 : end].key;         // of the windows that follow, one per lane
+  const int64_t r = a.rank ? (int64_t)a.rank[i1 - 1 < end ? i1 - 1 : end] : (int64_t)key;
+  if (i1 < a.n && key != a.none && next == key && !(i0 > 0 && prev == key)) {       // (the same in the team's lanes)
+    int terms = 1;              // the window's own sum, and one of each window that begins inside the run
+    for (int t0 = 1; t0 <= JOIN_SHORT; t0 += lanes) {
+      const int64_t f = (w + t0 + tl) * a.window;
+      const uint64_t m = __ballot(f < a.n && (t0 == 1 ? later : a.s[f < end ? f : end].key) == key);
+      const uint64_t of_team = lanes == 64 ? m : (m >> (threadIdx.x & 63 & ~(lanes - 1))) & ((1ULL << lanes) - 1);
+      const int in = __popcll(of_team);
+      terms += in;
+      if (in < lanes) break;
+    }
+    if (terms <= JOIN_SHORT) {
+      write(r, sum(w, 0, terms));
+    } else if (tl == 0) {
+      const int q = atomicAdd(&queued, 1);
+      queue[q].w = w;
+      queue[q].r = r;
+      queue[q].key = key;
     }
   }
   __syncthreads();
   const int todo = queued;
   for (int q = 0; q < todo; ++q) {                // (the order of the queue does not matter: its runs are independent)
-    const int64_t w = queue[q];
-    const uint32_t key = a.s[(w + 1) * a.window - 1].key;
+    const int64_t w = queue[q].w;
     int64_t terms = 1;
     for (;;) {
       const int64_t f = (w + terms + threadIdx.x) * a.window;
-      const int m = __syncthreads_count(f < a.n && a.s[f].key == key);
+      const int m = __syncthreads_count(f < a.n && a.s[f].key == queue[q].key);
       terms += m;
-      if (m < 256) break;
+      if (m < JOIN_THREADS) break;
     }
     const int64_t each = ceil_div64(terms, teams), b = team * each, e = b + each < terms ? b + each : terms;
     share[threadIdx.x] = sum(w, b, e);
@@ -578,7 +599,7 @@ __global__ __launch_bounds__(256) void k_segment_join(seg_args a) {
         const float4 v = share[(t << a.log_l) + tl];
         acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
       }
-      write(w, key, acc);
+      write(queue[q].r, acc);
     }
     __syncthreads();
   }
@@ -1083,10 +1104,10 @@ int launch_sums(seg_args a, bool accumulate, hipStream_t stream) {
   a.chunks = (a.width + 3) / 4;
   a.log_l = log_lanes(a.chunks, 6);
   a.col_blocks = (int)ceil_div64(a.chunks, 1 << a.log_l);
-  const int64_t blocks = ceil_div64(windows - 1, 256 >> a.log_l) * a.col_blocks;
+  const int64_t blocks = ceil_div64(windows - 1, JOIN_THREADS >> a.log_l) * a.col_blocks;
   ORCA_REQUIRE(blocks < (1LL << 31), "orca_embedding_backward: %lld ids of width %d are too many for one call", (long long)a.n, a.width);
-  if (accumulate) k_segment_join<TO, true><<<(unsigned)blocks, 256, 0, stream>>>(a);
-  else k_segment_join<TO, false><<<(unsigned)blocks, 256, 0, stream>>>(a);
+  if (accumulate) k_segment_join<TO, true><<<(unsigned)blocks, JOIN_THREADS, 0, stream>>>(a);
+  else k_segment_join<TO, false><<<(unsigned)blocks, JOIN_THREADS, 0, stream>>>(a);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
