@@ -469,6 +469,17 @@ int orca_clip_grads(int n, void* const* grads, const int64_t* sizes, const uint8
 int orca_adam_step(int n, float* const* params, const float* const* grads, float* const* exp_avg,
                    float* const* exp_avg_sq, const int64_t* sizes, double lr, double beta1, double beta2, double eps,
                    int64_t step, void* stream);
+/* the same with every gradient multiplied by *grad_scale (a device float; NULL: 1) on the way: the coefficient that
+ * orca_grad_norm leaves clips without a pass over the gradients */
+int orca_adam_step_scaled(int n, float* const* params, const float* const* grads, float* const* exp_avg,
+                          float* const* exp_avg_sq, const int64_t* sizes, double lr, double beta1, double beta2, double eps,
+                          int64_t step, const float* grad_scale, void* stream);
+/* the same step for the rows ids[0 .. min(*count, room)) of a [num_rows, width] parameter whose row-sparse gradient
+ * orca_embedding_backward_rows left (fp32 rows): the other rows and their moments stay as they are (the moments do not decay in
+ * steps without a gradient).  ids are distinct; ids outside [0, num_rows) are skipped. */
+int orca_adam_rows(const int64_t* ids, const float* rows, const int32_t* count, int64_t room, int64_t num_rows, int64_t width,
+                   float* param, float* exp_avg, float* exp_avg_sq, double lr, double beta1, double beta2, double eps,
+                   int64_t step, const float* grad_scale, void* stream);
 
 /* ---- native step driver: model/tgn_model.py:95-147 with modules/embedding_module.py:154-182 ----- */
 

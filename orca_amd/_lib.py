@@ -117,6 +117,8 @@ SIGNATURES = {
     "orca_decoder_train_workspace_floats": (i64, [i64]),
     "orca_decoder_train": (i32, [vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "orca_adam_step": (i32, [i32, vp, vp, vp, vp, vp, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, i64, vp]),
+    "orca_adam_step_scaled": (i32, [i32, vp, vp, vp, vp, vp] + [ctypes.c_double] * 4 + [i64, vp, vp]),
+    "orca_adam_rows": (i32, [vp, vp, vp, i64, i64, i64, vp, vp, vp] + [ctypes.c_double] * 4 + [i64, vp, vp]),
     "orca_embedding_forward": (i32, [vp, i32, i64, i64, i64, vp, vp, i64, ctypes.c_float, vp, vp]),
     "orca_embedding_backward_workspace_bytes": (i64, [i64, i64, i64]),
     "orca_embedding_backward": (i32, [vp, i32, i64, vp, vp, i64, i64, i64, i64, ctypes.c_float, i32, vp, i32, i64, vp, i64, vp]),

@@ -1313,16 +1313,23 @@ class OrcaEngine:
       self._opt = torch.optim.Adam(self._opt_params.values(), lr=lr)
     return self._opt
 
-  def step_optimizer(self, grads):
-    """optimizer.step() of train.py:238 with the gradients of train_step, then refresh()."""
+  def step_optimizer(self, grads, max_norm=None):
+    """optimizer.step() of train.py:238 with the gradients of train_step, then refresh().  max_norm: the gradients are clipped to
+    that global norm first (torch.nn.utils.clip_grad_norm_ between the two calls of train.py:237-238; several ranks clip alike, the
+    gradients are summed before); returns the norm before clipping, a device scalar.  Fused: the coefficient is applied inside the
+    Adam launch and `grads` stays as it is; with torch.optim.Adam the gradients are clipped in place."""
     if self._opt_params is None:
-      self._opt.step(grads)
+      norm = self._opt.step(grads, max_norm)
     else:
+      norm = None
+      if max_norm is not None:
+        norm = ops.clip_grad_norm({k: grads.get(k) for k in self._opt_params}, max_norm)
       for k, p in self._opt_params.items():
         g = grads.get(k)
         p.grad = None if g is None else g.reshape(p.shape)
       self._opt.step()
     self.refresh(beside=True, _time_unchanged=not self.train_time_encoder)
+    return norm
 
   def _dev(self, x, dtype):
     if not isinstance(x, torch.Tensor):

@@ -654,7 +654,8 @@ def clip_grad_norm(grads, max_norm, flat=None):
 class FusedAdam:
   """torch.optim.Adam(params, lr) (train.py:180) as one launch per step (orca_adam_step): params is a dict name ->
   fp32 device tensor, updated in place; step(grads) takes a dict with (a subset of) the same names -- a parameter
-  without a gradient is skipped, as torch skips p.grad is None."""
+  without a gradient is skipped, as torch skips p.grad is None.  A RowGrad (fp32 rows) as a gradient updates its rows only: the
+  others and their moments stay as they are, as with torch.optim.SparseAdam."""
 
   def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8):
     self.params = {k: v for k, v in params.items()}
@@ -671,22 +672,41 @@ class FusedAdam:
       o += -(-v.numel() // 64) * 64
     self.steps = {k: 0 for k in self.params}       # torch counts steps per parameter (a skipped one does not advance)
 
-  def step(self, grads):
-    by_step = {}
+  def step(self, grads, max_norm=None):
+    """max_norm: the gradients are clipped to that global norm on the way (grad_norm over those that belong to a parameter; the
+    coefficient stays on the device, the gradients as they are).  Returns the norm before clipping, or None without max_norm."""
+    used = {}
     for k, p in self.params.items():
       g = grads.get(k)
       if g is None:
         continue
-      if g.numel() != p.numel() or g.dtype != torch.float32 or not g.is_cuda:
-        raise _lib.OrcaError(f"FusedAdam: gradient of {k} does not match its parameter")
+      if isinstance(g, RowGrad):
+        if p.dim() != 2 or g.rows.shape[1:] != p.shape[1:] or g.num_rows != p.shape[0] or g.rows.dtype != torch.float32 or not g.rows.is_cuda:
+          raise _lib.OrcaError(f"FusedAdam: row gradient of {k} does not match its parameter")
+        used[k] = g
+      else:
+        if g.numel() != p.numel() or g.dtype != torch.float32 or not g.is_cuda:
+          raise _lib.OrcaError(f"FusedAdam: gradient of {k} does not match its parameter")
+        used[k] = g.contiguous()
+    norm = coef = None
+    if max_norm is not None:
+      norm, coef = grad_norm(used, max_norm)
+    by_step = {}
+    for k, g in used.items():
       self.steps[k] += 1
-      by_step.setdefault(self.steps[k], []).append((p, g.contiguous(), self.exp_avg[k], self.exp_avg_sq[k]))
+      if isinstance(g, RowGrad):
+        check(_lib.load().orca_adam_rows(ptr(g.ids), ptr(g.rows), ptr(g.count), g.ids.numel(), g.num_rows, g.rows.shape[1], ptr(self.params[k]),
+                                         ptr(self.exp_avg[k]), ptr(self.exp_avg_sq[k]), self.lr, self.betas[0], self.betas[1], self.eps,
+                                         self.steps[k], ptr(coef), stream()), "orca_adam_rows")
+      else:
+        by_step.setdefault(self.steps[k], []).append((self.params[k], g, self.exp_avg[k], self.exp_avg_sq[k]))
     for t, lst in by_step.items():
       n = len(lst)
       arr = lambda j: (ctypes.c_void_p * n)(*[x[j].data_ptr() for x in lst])
       sizes = (ctypes.c_int64 * n)(*[x[0].numel() for x in lst])
-      check(_lib.load().orca_adam_step(n, arr(0), arr(1), arr(2), arr(3), sizes, self.lr, self.betas[0], self.betas[1],
-                                       self.eps, t, stream()), "orca_adam_step")
+      check(_lib.load().orca_adam_step_scaled(n, arr(0), arr(1), arr(2), arr(3), sizes, self.lr, self.betas[0], self.betas[1],
+                                              self.eps, t, ptr(coef), stream()), "orca_adam_step")
+    return norm
 
 
 def find_uncached(nbr, batch_nodes, cache_flag, slot, epoch, bitmap):

@@ -116,3 +116,14 @@ def test_clip_refusals(norm_only):
   bad("width", rows=(P,), widths=(0,))
   if not norm_only:
     bad("no flat buffer", flat=(0, P, P))
+
+
+def test_adam_rows_refusals():
+  def rows(ids=P, g=P, count=P, room=3, num_rows=4, width=8, p=P, m=P, v=P, step=1):
+    return _lib.load().orca_adam_rows(ids, g, count, room, num_rows, width, p, m, v, 1e-3, 0.9, 0.999, 1e-8, step, None, None)
+  for bad in (dict(room=-1), dict(room=1 << 31), dict(num_rows=-1), dict(width=0), dict(step=0)):
+    refused(rows(**bad), "bad sizes")
+  for bad in ("ids", "g", "count", "p", "m", "v"):
+    refused(rows(**{bad: None}), "null argument")
+  assert rows(room=0, ids=None) == 0
+  refused(_lib.load().orca_adam_step_scaled(1, None, None, None, None, None, 1e-3, 0.9, 0.999, 1e-8, 1, None, None), "bad arguments")
