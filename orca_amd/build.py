@@ -10,14 +10,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "liborca_hip.so")
 HOST = os.path.join(HERE, "_host.so")      # csrc/bind.cpp: torch tensors -> C ABI for the calls where the host's time counts
-SOURCES = ["csr.hip", "tgat.hip", "tgat_bwd.hip", "gru_bwd.hip", "gru.hip", "state.hip", "plan.hip", "plan_dev.hip", "engine.hip", "optim.hip", "clip.hip", "embedding.hip", "decoder.hip"]
+SOURCES = ["csr.hip", "tgat.hip", "tgat_bwd.hip", "gru_bwd.hip", "gru.hip", "state.hip", "plan.hip", "plan_dev.hip", "engine.hip", "optim.hip", "clip.hip", "clip_adam.hip", "embedding.hip", "decoder.hip"]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-Wall",
          "-Wno-unused-result", "-Wno-unused-function"]
 
 
 # no packed fp32 instructions in the sources that carry this (some of their forms have given wrong results on gfx950)
 NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SCALAR_FP32 = {"clip.hip", "embedding.hip"}
+SCALAR_FP32 = {"clip.hip", "clip_adam.hip", "embedding.hip"}
 
 
 def _stale(target, deps):
