@@ -4,7 +4,7 @@
 // adds those sums up in the same order (while its first piece is on its way) before it scales its share.  Squares and sums are fp64:
 // neither overflows nor vanishes for any fp32 input, and the conversions hide behind the loads (4.5 elements per clock and CU at the
 // HBM rate for 16-bit gradients).
-//   A list travels in the kernel's arguments, under 4 KB: 12 bytes per tensor (20 with flat buffers), so that a few hundred tensors
+//   A list travels in the kernel's arguments, under 4 KB: 12 bytes per tensor (16 with flat buffers), so that a few hundred tensors
 // are one launch.  With a search by scalar loads through 41 bytes per tensor, k_norm_partial took 6.4 us for 32 tensors of 2.9 MB.
 #include <algorithm>
 #include "elem.h"
@@ -15,7 +15,7 @@ constexpr int PIECE = 16384, SMALL_PIECE = 4096;        // bytes a workgroup tak
 // 60 MB 33.1 against 31.6 with plain accesses, 120 MB 59.7 (71.9), 300 MB 142 (174), 1 GB 484 (552).
 constexpr int64_t STREAM_BYTES = 100000000;
 constexpr int PARTS = 2048;           // most partial sums of a call
-constexpr int SPARSE_MAX = 8;         // row-sparse tensors per launch
+constexpr int SPARSE_MAX = 4;         // row-sparse tensors per launch
 
 struct sparse_grad {
   const int32_t* rows;                // the device count
@@ -29,11 +29,11 @@ template <int N, bool FLAT> struct grad_list {
   int first[N + 1];                   // first piece of each tensor
   int which[SPARSE_MAX];              // the tensors that are row-sparse
   sparse_grad sparse[SPARSE_MAX];
-  int64_t to[FLAT ? N : 1];           // flat: where the tensor begins in its type's buffer, in elements
-  char* flat[3];
+  uint32_t to[FLAT ? N : 1];          // flat: where the tensor begins in its type's buffer, in elements from flat[type]
+  char* flat[3];                      // (the buffers, moved on to this list's first tensor of the type)
 };
-typedef grad_list<300, false> in_place_list;
-typedef grad_list<180, true> flat_list;
+typedef grad_list<310, false> in_place_list;
+typedef grad_list<235, true> flat_list;
 static_assert(sizeof(in_place_list) <= 4000 && sizeof(flat_list) <= 4000, "kernel arguments");
 
 struct piece { char* p; int64_t offset; int len, dtype, tensor; };       // offset: bytes from the tensor's beginning
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256) void k_clip(L list, const double* __restrict__
   if (!FLAT && c == 1.0f) return;
   for (;;) {
     char* out = q.p + q.offset;
-    if constexpr (FLAT) out = list.flat[q.dtype] + list.to[q.tensor] * (q.dtype == ORCA_F32 ? 4 : 2) + q.offset;
+    if constexpr (FLAT) out = list.flat[q.dtype] + (int64_t)list.to[q.tensor] * (q.dtype == ORCA_F32 ? 4 : 2) + q.offset;
     if (q.dtype == ORCA_F32) scale<STREAMS, float>(r, q, out, c);
     else if (q.dtype == ORCA_BF16) scale<STREAMS, __bf16>(r, q, out, c);
     else scale<STREAMS, _Float16>(r, q, out, c);
@@ -233,16 +233,18 @@ int check_list(const char* who, host_list* h, double max_norm, const float* norm
   return ORCA_OK;
 }
 
-// The list from tensor *i on, as much of it as a launch takes.  `to`: elements of each type so far (flat buffers), moved on.
+// The list from tensor *i on, as much of it as a launch takes.  `to`: elements of each type so far, moved on.
 template <class L, bool FLAT> void take(const host_list& h, int* i, int64_t* to, L* list) {
   constexpr int N = (int)(sizeof(L::at) / 8);
   list->n = list->n_sparse = 0;
-  int64_t pieces = 0;
+  int64_t pieces = 0, from[3] = {0, 0, 0};
+  if constexpr (FLAT) std::copy(to, to + 3, from);
   for (; *i < h.n && list->n < N; ++*i) {
     if (h.sizes[*i] == 0) continue;
     const int t = list->n, dt = h.dtypes[*i];
     const bool sparse = h.rows && h.rows[*i];
     if (sparse && list->n_sparse == SPARSE_MAX) break;
+    if (FLAT && to[dt] - from[dt] >= (1LL << 32)) break;
     const int64_t bytes = bytes_of(h, *i), mine = ceil_div64(bytes, h.piece);
     const uint64_t tail = (uint64_t)(bytes - (mine - 1) * h.piece);
     list->at[t] = (uint64_t)(uintptr_t)h.grads[*i] | (tail / 2 - 1) << 48 | (uint64_t)sparse << 61 | (uint64_t)dt << 62;
@@ -251,7 +253,7 @@ template <class L, bool FLAT> void take(const host_list& h, int* i, int64_t* to,
       list->sparse[list->n_sparse++] = sparse_grad{h.rows[*i], h.widths[*i], dt};
     }
     if constexpr (FLAT) {
-      list->to[t] = to[dt];
+      list->to[t] = (uint32_t)(to[dt] - from[dt]);
       to[dt] += h.sizes[*i];
     }
     list->first[t] = (int)pieces;
@@ -284,10 +286,10 @@ int clip(const host_list& h, void* const* flat, const double* part, int parts, d
   int64_t to[3] = {0, 0, 0};
   for (int i = 0; i < h.n;) {
     L list;
+    if constexpr (FLAT)
+      for (int k = 0; k < 3; ++k) list.flat[k] = (char*)flat[k] + to[k] * (k == ORCA_F32 ? 4 : 2);
     take<L, FLAT>(h, &i, to, &list);
     if (list.n == 0) continue;
-    if constexpr (FLAT)
-      for (int k = 0; k < 3; ++k) list.flat[k] = (char*)flat[k];
     const unsigned grid = (unsigned)std::min(list.first[list.n], 2048);
     if (h.piece == SMALL_PIECE) k_clip<SMALL_PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, part, parts, max_norm, norm);
     else if (FLAT && h.pieces * h.piece > STREAM_BYTES) k_clip<PIECE, FLAT, L, FLAT><<<grid, 256, 0, stream>>>(list, part, parts, max_norm, norm);
