@@ -206,13 +206,16 @@ __global__ __launch_bounds__(64) void k_sort_columns(uint32_t* __restrict__ coun
   totals[b] = run;
 }
 
-__device__ __forceinline__ uint32_t wave_inclusive(uint32_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
+// inclusive prefix sums over the wave: within rows of 16 by row shifts, then the rows' last lanes broadcast (no LDS round trips)
+__device__ __forceinline__ uint32_t wave_inclusive(uint32_t v) {
+  int x = (int)v;
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return (uint32_t)x;
 }
 
 // the lanes of `in` whose digit equals this lane's: per bit one compare, and one three-operand bit operation per half of the mask
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
   }
   // exclusive prefix of the totals over the bins
   const uint32_t mine = total[0] + total[1] + total[2] + total[3];
-  const uint32_t inc = wave_inclusive(mine, lane);
+  const uint32_t inc = wave_inclusive(mine);
   if (lane == 63) wave_sum[wave] = inc;
   __syncthreads();
   uint32_t run = inc - mine;
@@ -622,7 +625,7 @@ constexpr int64_t SMALL_VALUES = 1 << 20;      // beyond, a hub id's rows are to
 constexpr int SMALL_MAP = 65536;               // table rows of a workgroup's share, at most (bits in LDS)
 constexpr int SMALL_RUN = 32;                  // a longer run of equal ids is added by the whole workgroup ...
 constexpr int SMALL_TEAMS = 32;                // ... in at most this many consecutive parts
-constexpr int SMALL_PAIRS = 128;               // up to this many pairs are sorted by counting the smaller ones, one thread per pair
+constexpr int SMALL_PAIRS = 512;               // up to this many pairs (and a thread each) are sorted by counting the smaller ones
 constexpr int SMALL_DIGIT = 8;                 // digit bits of the sort of longer lists
 constexpr int MAX_RANGES = 256;
 struct small_args {
@@ -640,7 +643,7 @@ struct small_args {
 struct small_lds { int region, heads, bytes; };
 __host__ __device__ inline small_lds small_layout(int threads, int n) {
   small_lds l;
-  l.region = (n + (n & 1)) * 8;
+  l.region = (n + 63) / 64 * 64 * 8;
   l.heads = l.region + threads * 8 * 4;
   l.bytes = l.heads + 2 * (n + 1);
   return l;
@@ -692,20 +695,35 @@ template <int THREADS>
 __device__ __forceinline__ void small_sort(pair32* list, int m, uint32_t least, int bits, char* region, uint32_t* wave_sum) {
   constexpr int WAVES = THREADS / 64;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  if (m <= SMALL_PAIRS) {
-    static_assert(SMALL_PAIRS == 128, "two waves of pairs");
-    pair32 p{0u, ~0u};
-    int rank = 0;
-    if (wave < 2) {
-      const uint32_t lo = lane < m ? list[lane].key : ~0u, hi = 64 + lane < m ? list[64 + lane].key : ~0u;
-      if (t < m) p = pair32{list[t].pos, wave ? hi : lo};
-      for (int j = 0; j < min(m, 64); ++j) {
-        const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)lo, j);
-        rank += key < p.key || (key == p.key && j < t);
-      }
-      for (int j = 64; j < m; ++j) {
-        const uint32_t key = (uint32_t)__builtin_amdgcn_readlane((int)hi, j - 64);
-        rank += key < p.key || (key == p.key && j < t);
+  if (m <= min(SMALL_PAIRS, THREADS)) {
+    // the keys come four at a time out of LDS, the same for all lanes; a block of 64 pairs before this wave's also counts its equals
+    const pair32 p = t < m ? list[t] : pair32{0u, ~0u};
+    if (t >= m && t < (m + 63) / 64 * 64) list[t].key = ~0u;
+    __syncthreads();
+    uint32_t rank = 0;
+    if (wave * 64 < m) {
+      for (int b = 0; b * 64 < m; ++b) {
+        const u32x4* two = reinterpret_cast<const u32x4*>(list + 64 * b);
+        const int half = (min(64, m - 64 * b) + 1) / 2;
+        if (b < wave) {
+#pragma unroll 8
+          for (int j = 0; j < 32; ++j) {
+            const u32x4 v = two[j];
+            rank += (uint32_t)(v[1] <= p.key) + (uint32_t)(v[3] <= p.key);
+          }
+        } else if (b > wave) {
+#pragma unroll 4
+          for (int j = 0; j < half; ++j) {
+            const u32x4 v = two[j];
+            rank += (uint32_t)(v[1] < p.key) + (uint32_t)(v[3] < p.key);
+          }
+        } else {
+#pragma unroll 4
+          for (int j = 0; j < half; ++j) {
+            const u32x4 v = two[j];
+            rank += (uint32_t)(v[1] < p.key || (v[1] == p.key && 2 * j < lane)) + (uint32_t)(v[3] < p.key || (v[3] == p.key && 2 * j + 1 < lane));
+          }
+        }
       }
     }
     __syncthreads();
@@ -753,7 +771,7 @@ __device__ __forceinline__ void small_sort(pair32* list, int m, uint32_t least, 
         total += c[w];
       }
     }
-    const uint32_t mine = (total & 0xffff) + (total >> 16), inc = wave_inclusive(mine, lane);
+    const uint32_t mine = (total & 0xffff) + (total >> 16), inc = wave_inclusive(mine);
     uint32_t all;
     const uint32_t run = small_offsets<THREADS>((uint32_t)__builtin_amdgcn_readlane((int)inc, 63), wave_sum, &all) + inc - mine;
     if (2 * t < bins) {
@@ -847,6 +865,7 @@ __device__ __forceinline__ void small_sums(const small_args& a, int runs, B begi
       }
       __syncthreads();
       if (team == 0 && live) {
+#pragma unroll 4
         for (int k = 1; k < most; ++k)
 #pragma unroll
           for (int j = 0; j < VEC; ++j) acc[j] += parts[((k << a.log_l) + tl) * VEC + j];
@@ -955,16 +974,15 @@ __global__ __launch_bounds__(THREADS) void k_range_sort(small_args a, range_work
   small_keys<THREADS>(a, base, items, key);
   const uint32_t lo = (uint32_t)(a.num_rows * (int64_t)blockIdx.x / gridDim.x), hi = (uint32_t)(a.num_rows * (int64_t)(blockIdx.x + 1) / gridDim.x);
   uint64_t take[SMALL_ITEMS];
-  uint32_t mine = 0, below = 0, m, before;
+  uint32_t mine = 0, both;            // what is below the range is counted in the upper half (at most SMALL_N in each)
 #pragma unroll
   for (int u = 0; u < SMALL_ITEMS; ++u) {
     if (u >= items) break;
     take[u] = __ballot(key[u] >= lo && key[u] < hi);
-    mine += (uint32_t)__popcll(take[u]);
-    below += (uint32_t)__popcll(__ballot(key[u] < lo));
+    mine += (uint32_t)__popcll(take[u]) + ((uint32_t)__popcll(__ballot(key[u] < lo)) << 16);
   }
-  uint32_t run = small_offsets<THREADS>(mine, wave_sum, &m);
-  small_offsets<THREADS>(below, wave_sum, &before);
+  uint32_t run = small_offsets<THREADS>(mine, wave_sum, &both) & 0xffff;
+  const uint32_t m = both & 0xffff, before = both >> 16;
 #pragma unroll
   for (int u = 0; u < SMALL_ITEMS; ++u) {
     if (u >= items) break;
@@ -988,55 +1006,52 @@ __global__ __launch_bounds__(THREADS) void k_range_sort(small_args a, range_work
   }
 }
 
-template <class TI, class TO, int VEC>
-__global__ __launch_bounds__(TINY_THREADS) void k_range_sums(small_args a, range_work w, int ranges, int64_t* __restrict__ ids, int32_t* __restrict__ count) {
-  __shared__ uint32_t wave_sum[TINY_THREADS / 64], queue[64], row[MAX_RANGES + 1], first[MAX_RANGES + 1];
+constexpr int RANGE_RUNS = 64;        // runs whose places are looked up together
+template <int THREADS, class TI, class TO, int VEC>
+__global__ __launch_bounds__(THREADS) void k_range_sums(small_args a, range_work w, int ranges, int64_t* __restrict__ ids, int32_t* __restrict__ count) {
+  __shared__ uint32_t wave_sum[THREADS / 64], queue[64], row[MAX_RANGES + 1], first[MAX_RANGES + 1], begin[RANGE_RUNS + 1], key[RANGE_RUNS];
   __shared__ int queued;
-  __shared__ float parts[TINY_THREADS * 8];
-  static_assert(MAX_RANGES == TINY_THREADS, "a thread per range");
+  __shared__ float parts[THREADS * 8];
+  static_assert(MAX_RANGES <= THREADS, "a thread per range");
   const int t = threadIdx.x, lane = t & 63;
-  const uint32_t mine = t < ranges ? w.distinct[t] : 0u, inc = wave_inclusive(mine, lane);
-  first[t] = t <= ranges ? w.first[t] : 0u;
-  if (t == 0) {
-    queued = 0;
-    if (ranges == MAX_RANGES) first[MAX_RANGES] = w.first[MAX_RANGES];
-  }
+  const uint32_t mine = t < ranges ? w.distinct[t] : 0u, inc = wave_inclusive(mine);
+  if (t <= MAX_RANGES) first[t] = t <= ranges ? w.first[t] : 0u;
+  if (THREADS == MAX_RANGES && t == 0 && ranges == MAX_RANGES) first[MAX_RANGES] = w.first[MAX_RANGES];
+  if (t == 0) queued = 0;
   uint32_t all;
-  const uint32_t run = small_offsets<TINY_THREADS>((uint32_t)__builtin_amdgcn_readlane((int)inc, 63), wave_sum, &all) + inc - mine;
-  row[t] = run;                 // rows of the ranges before
+  const uint32_t run = small_offsets<THREADS>((uint32_t)__builtin_amdgcn_readlane((int)inc, 63), wave_sum, &all) + inc - mine;
+  if (t < MAX_RANGES) row[t] = run;                 // rows of the ranges before
   if (t == 0) row[MAX_RANGES] = all;
   __syncthreads();
   if (blockIdx.x == 0 && t == 0) *count = (int32_t)all;
   const int share = (int)(gridDim.x / (uint32_t)a.col_blocks), sh = (int)(blockIdx.x / (uint32_t)a.col_blocks);
-  const int r0 = (int)((int64_t)all * sh / share), r1 = (int)((int64_t)all * (sh + 1) / share);
-  auto range_of = [&](int r) {          // the range that holds row r0 + r: row[range] <= r0 + r < row[range + 1]
-    int lo = 0;
+  const int r1 = (int)((int64_t)all * (sh + 1) / share);
+  for (int r0 = (int)((int64_t)all * sh / share); r0 < r1; r0 += RANGE_RUNS) {
+    const int runs = min(RANGE_RUNS, r1 - r0);
+    if (t <= runs) {            // where run r0 + t begins; the last one's end is where the next one would
+      int k = 0;                // its range: row[k] <= r0 + t < row[k + 1]
 #pragma unroll
-    for (int step = MAX_RANGES / 2; step; step >>= 1) lo += (int)row[lo + step] <= r0 + r ? step : 0;
-    return lo;
-  };
-  auto begin = [&](int r) {
-    const int k = range_of(r);
-    return (int)(first[k] + w.heads[first[k] + (uint32_t)(r0 + r) - row[k]]);
-  };
-  auto end = [&](int r) {
-    const int k = range_of(r);
-    const bool last = (uint32_t)(r0 + r) + 1 == row[k + 1];
-    return (int)(last ? first[k + 1] : first[k] + w.heads[first[k] + (uint32_t)(r0 + r) - row[k] + 1]);
-  };
-  small_sums<TINY_THREADS, TI, VEC>(
-      a, r1 - r0, begin, end, [&](int k) { return w.pos[k]; },
-      [&](int r, const float (&acc)[VEC], int col, int own) {
-        if (col == 0) {
-          const int k = range_of(r);
-          ids[r0 + r] = (int64_t)w.key[first[k] + (uint32_t)(r0 + r) - row[k]];
-        }
-        float f[VEC];
+      for (int step = MAX_RANGES / 2; step; step >>= 1) k += (int)row[k + step] <= r0 + t ? step : 0;
+      const bool none = (uint32_t)(r0 + t) >= all;
+      const uint32_t at = first[k] + (uint32_t)(r0 + t) - row[k];
+      begin[t] = none ? first[ranges] : first[k] + w.heads[at];
+      if (t < runs) key[t] = w.key[at];
+    }
+    __syncthreads();
+    small_sums<THREADS, TI, VEC>(
+        a, runs, [&](int r) { return (int)begin[r]; }, [&](int r) { return (int)begin[r + 1]; }, [&](int k) { return w.pos[k]; },
+        [&](int r, const float (&acc)[VEC], int col, int own) {
+          if (col == 0) ids[r0 + r] = (int64_t)key[r];
+          float f[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = acc[j] * a.scale;
-        store_chunk<VEC, TO>((TO*)a.out + (int64_t)(r0 + r) * a.ld_out + col, f);
-      },
-      parts, queue, &queued);
+          for (int j = 0; j < VEC; ++j) f[j] = acc[j] * a.scale;
+          store_chunk<VEC, TO>((TO*)a.out + (int64_t)(r0 + r) * a.ld_out + col, f);
+        },
+        parts, queue, &queued);
+    __syncthreads();
+    if (t == 0) queued = 0;
+    __syncthreads();
+  }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -1177,11 +1192,13 @@ int small_rows(small_args a, char* ws, int64_t* ids, int32_t* count, hipStream_t
   const range_work w = range_layout(ws, a.n, &bytes);
   const int ranges = (int)std::min<int64_t>(MAX_RANGES, ceil_div64(a.n, 4));
   if (int rc = a.n <= TINY_N ? launch_range_sort<TINY_THREADS>(a, w, ranges, stream) : launch_range_sort<SMALL_THREADS>(a, w, ranges, stream)) return rc;
-  // a run per team and workgroup, at most two workgroups per CU (and one for each column block)
-  const int64_t shares = std::max<int64_t>(1, std::min(ceil_div64(a.n, TINY_THREADS >> a.log_l), ceil_div64(512, a.col_blocks)));
+  // a run per team and workgroup, at most 1024 teams' waves per CU (and a workgroup for each column block)
+  const int threads = a.n <= TINY_N ? TINY_THREADS : SMALL_THREADS;
+  const int64_t shares = std::max<int64_t>(1, std::min(ceil_div64(a.n, threads >> a.log_l), ceil_div64(a.n <= TINY_N ? 512 : 256, a.col_blocks)));
   const unsigned grid = (unsigned)(shares * a.col_blocks);
-  if (a.width >= VEC) k_range_sums<TI, TO, VEC><<<grid, TINY_THREADS, 0, stream>>>(a, w, ranges, ids, count);
-  else k_range_sums<TI, TO, 1><<<grid, TINY_THREADS, 0, stream>>>(a, w, ranges, ids, count);
+  auto* kernel = a.n <= TINY_N ? (a.width >= VEC ? k_range_sums<TINY_THREADS, TI, TO, VEC> : k_range_sums<TINY_THREADS, TI, TO, 1>)
+                               : (a.width >= VEC ? k_range_sums<SMALL_THREADS, TI, TO, VEC> : k_range_sums<SMALL_THREADS, TI, TO, 1>);
+  kernel<<<grid, (unsigned)threads, 0, stream>>>(a, w, ranges, ids, count);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
