@@ -645,7 +645,7 @@ def clip_grad_norm(grads, max_norm, flat=None):
   """orca_clip_grads: grad_norm(grads), and every gradient scaled by min(1, max_norm / (norm + 1e-6)) as torch.nn.utils.clip_grad_norm_
   does (product in fp32, one rounding; a norm that is not finite makes the gradients NaN or 0 as there).  In place, or with flat = a
   contiguous tensor for each type among the gradients (in the order in which the types first appear), where the products of that
-  type's gradients go one after another and the gradients stay as they are.  Returns the norm before clipping as a float32 scalar
+  type's gradients go one after another and the gradients stay as they are.  The tensors must not overlap.  Returns the norm before clipping as a float32 scalar
   tensor; nothing is read by the host."""
   return (_host or _load_host()).clip_grad_norm(list(grads.values() if isinstance(grads, dict) else grads), max_norm,
                                                 None if flat is None else list(flat))

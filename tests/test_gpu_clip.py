@@ -167,6 +167,40 @@ def test_row_sparse_gradients(ops, dtype, count):
   assert bool(rows[count:].isnan().all())
 
 
+def test_many_row_sparse_gradients(ops):
+  """more of them than one launch takes, between dense ones"""
+  g = torch.Generator().manual_seed(7)
+  rgs = [ops.RowGrad(torch.arange(50, device=DEV), torch.randn(50, 9 + i, generator=g).to(DEV),
+                     torch.tensor([3 * i], dtype=torch.int32, device=DEV), 100) for i in range(11)]
+  dense = make([4097, 3, 20000], TYPES[:1])
+  lst = [dense[0]] + rgs[:6] + [dense[1]] + rgs[6:] + [dense[2]]
+  keep = [r.rows.clone() for r in rgs]
+  want = norm64([r.rows[:3 * i] for i, r in enumerate(rgs)] + dense)
+  check_norm(ops.grad_norm(lst), want)
+  flat = torch.full((sum(r.rows.numel() for r in rgs) + sum(d.numel() for d in dense),), 6.0, device=DEV)
+  check_norm(ops.clip_grad_norm(lst, 0.5, flat=[flat]), want)
+  c, at = 0.5 / (want + 1e-6), dense[0].numel()
+  for i, r in enumerate(rgs):
+    n, live = r.rows.numel(), 3 * i * r.rows.shape[1]
+    check_scaled(flat[at:at + live].view(3 * i, -1) if i else flat[:0].view(0, 9), keep[i][:3 * i], c)
+    assert bool((flat[at + live:at + n] == 6).all())
+    at += n + (dense[1].numel() if i == 5 else 0)
+  check_norm(ops.clip_grad_norm(lst, 0.5), want)
+  for i, r in enumerate(rgs):
+    check_scaled(r.rows[:3 * i], keep[i][:3 * i], c)
+    assert torch.equal(r.rows[3 * i:], keep[i][3 * i:])
+
+
+def test_large_flat_copy(ops):
+  """a list of 120 MB: read and written past the caches"""
+  grads = [torch.randn(s, generator=torch.Generator(device=DEV).manual_seed(s), device=DEV) * 0.01 for s in (20_000_001, 9_999_999, 5)]
+  flat = torch.empty(sum(x.numel() for x in grads), device=DEV)
+  want = norm64(grads)
+  check_norm(ops.clip_grad_norm(grads, 1.0, flat=[flat]), want)
+  exp = torch.cat(grads).double() * (1.0 / (want + 1e-6))
+  assert bool(((flat.double() - exp).abs() <= 1.01 * 3 * U * exp.abs() + 1e-45).all())
+
+
 def test_captured_and_replayed(ops):
   grads = make([100, 40000, 3, 9001], TYPES)
   flat = [torch.empty(sum(x.numel() for x in grads if x.dtype is t), dtype=t, device=DEV) for t in dict.fromkeys(x.dtype for x in grads)]

@@ -184,6 +184,60 @@ def test_long_run_over_many_tiles(ops):
     check_grad(got, grad, i, vocab, 1.0, None)
 
 
+@pytest.mark.parametrize("width", [1, 3, 4, 7, 8, 17, 100, 129, 257, 1030])
+@pytest.mark.parametrize("g_type,o_type", [(torch.float32, None), (torch.bfloat16, None), (torch.float16, None), (torch.bfloat16, torch.float32)])
+def test_long_lists_widths_and_types(ops, width, g_type, o_type):
+  """more ids than a short list has: the windows' sums and their joins, accumulated into a strided table, and the row-sparse form"""
+  n, vocab = 8193 + width % 5, 700
+  ids = make_ids("hubs", n, vocab, width, torch.int32).to(DEV)
+  grad = torch.randn(n, width, generator=torch.Generator().manual_seed(width)).to(g_type).to(DEV)
+  got = ops.embedding_backward(grad, ids, vocab, scale=0.5, padding_idx=3, dtype=o_type)
+  check_grad(got, grad, ids, vocab, 0.5, 3)
+  rg = ops.embedding_backward_rows(grad, ids, vocab, scale=0.5, padding_idx=3, dtype=o_type)
+  k = int(rg.count)
+  assert torch.equal(rg.rows[:k], got[rg.ids[:k]]) and bool((rg.ids[:k] != 3).all())
+  base = torch.full((vocab, width + 3), 2.0, dtype=got.dtype, device=DEV)
+  out = base[:, 1:1 + width]
+  start = torch.randn(vocab, width, generator=torch.Generator().manual_seed(4)).to(got.dtype).to(DEV)
+  out.copy_(start)
+  ops.embedding_backward(grad, ids, vocab, scale=0.5, padding_idx=3, out=out, accumulate=True)
+  G, S, m = reference(grad, ids, vocab, 0.5, 3)
+  exp = start.cpu().double() + G
+  lim = 1.01 * ((m[:, None] + 2) * U * S + (half(out.dtype) + U) * exp.abs()) + tiny(out.dtype)
+  assert bool(((out.cpu().double() - exp).abs() <= lim).all())
+  assert bool((base[:, 0] == 2).all()) and bool((base[:, 1 + width:] == 2).all()), "what lies between the rows"
+  out.fill_(9)
+  assert torch.equal(ops.embedding_backward(grad, ids, vocab, scale=0.5, padding_idx=3, out=out), got)
+  assert bool((base[:, 0] == 2).all()) and bool((base[:, 1 + width:] == 2).all())
+
+
+def test_few_ids_in_a_tall_table(ops):
+  """more rows than the short list's workgroups can mark: the zeros come from the sort's launches"""
+  V = 17_000_003
+  ids = torch.tensor([0, V - 1, 5, V - 1, 16_777_216, -7, V], device=DEV)
+  got = ops.embedding_backward(torch.arange(1.0, 8.0, device=DEV)[:, None], ids, V)
+  assert got[[0, 5, 16_777_216, V - 1], 0].tolist() == [1.0, 3.0, 5.0, 6.0] and int((got != 0).sum()) == 4
+  got.fill_(1.0)
+  ops.embedding_backward(torch.ones(7, 1, device=DEV), ids, V, out=got, accumulate=True)
+  assert got[[0, 5, 16_777_216, V - 1, 1], 0].tolist() == [2.0, 2.0, 2.0, 3.0, 1.0]
+
+
+def test_large_gradients_and_tables(ops):
+  """the accesses past the caches: 150 MB of gradient rows, a table of 420 MB"""
+  n, w, vocab = 73_000, 1024, 205_000
+  g = torch.Generator(device=DEV).manual_seed(1)
+  grad = torch.empty(n, w, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+  ids = (torch.rand(n, generator=g, device=DEV) ** 3 * vocab).long()
+  got = ops.embedding_backward(grad, ids, vocab, scale=2.0)
+  G = torch.zeros(vocab, w, device=DEV, dtype=torch.float64).index_add_(0, ids, grad.double()).mul_(2.0)
+  S = torch.zeros(vocab, w, device=DEV, dtype=torch.float64).index_add_(0, ids, grad.double().abs()).mul_(2.0)
+  m = torch.bincount(ids, minlength=vocab)[:, None]
+  assert bool(((got.double() - G).abs() <= 1.01 * ((m + 2) * U * S + half(torch.bfloat16) * G.abs()) + tiny(torch.bfloat16)).all())
+  rg = ops.embedding_backward_rows(grad, ids, vocab, scale=2.0)
+  k = int(rg.count)
+  assert torch.equal(rg.rows[:k], got[rg.ids[:k]])
+
+
 def test_empty_and_all_padding(ops):
   e = torch.empty(0, 8, device=DEV)
   none = torch.empty(0, dtype=torch.int64, device=DEV)
