@@ -109,7 +109,7 @@ int embedding_typed(const void* table, int64_t n_rows, int64_t width, int64_t ld
 // ---- zeros ahead of the sums -----------------------------------------------------------------------------------------
 // A dense gradient starts as zeros; nothing before the sums reads it, so the launches of the sort carry the zero fill in extra
 // workgroups: the sort waits on latency with a few dozen workgroups, the fill on the HBM, and the longer of the two is what counts.
-constexpr int FILL_PIECE = 32768;       // bytes a workgroup writes at a time
+constexpr int FILL_PIECE = 16384;       // bytes a workgroup writes: few and in order (400 MB in pieces of 32 KB 74 us, of 16 KB, a store per thread 60)
 struct fill_job {
   char* p;                      // `rows` rows of `bytes` bytes, `pitch` bytes apart (a table without gaps is one row)
   int64_t bytes, pitch, per_row, from, to;      // pieces of a row; this launch's pieces
@@ -137,7 +137,7 @@ template <int THREADS> __device__ __forceinline__ void fill_pieces(const fill_jo
   if (f.past) fill_loop<THREADS, true>(f, block, blocks);
   else fill_loop<THREADS, false>(f, block, blocks);
 }
-__global__ __launch_bounds__(512) void k_fill(fill_job f) { fill_pieces<512>(f, blockIdx.x, gridDim.x); }
+__global__ __launch_bounds__(1024) void k_fill(fill_job f) { fill_pieces<1024>(f, blockIdx.x, gridDim.x); }
 
 // ---- sort of the positions by id -------------------------------------------------------------------------------------
 // Stable least-significant-digit radix sort of (key, position) pairs; key = the id, or num_rows for what has no row (the padding
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(256) void k_segment_sum(seg_args a) {
 // The runs that cross window borders, each taken by the window that begins it: sum of what that window and the following ones left in
 // `part`, in their order.  A team takes one window; a run over more than JOIN_SHORT windows is left to the whole workgroup, whose teams
 // take a consecutive share of the terms each.
-constexpr int JOIN_SHORT = 16, JOIN_THREADS = 1024;
+constexpr int JOIN_SHORT = 16, JOIN_THREADS = 1024, JOIN_TEAMS = 32;
 template <class TO, bool ACCUMULATE>
 __global__ __launch_bounds__(JOIN_THREADS) void k_segment_join(seg_args a) {
   __shared__ float4 share[JOIN_THREADS];
@@ -593,12 +593,14 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_segment_join(seg_args a) {
       terms += m;
       if (m < JOIN_THREADS) break;
     }
-    const int64_t each = ceil_div64(terms, teams), b = team * each, e = b + each < terms ? b + each : terms;
-    share[threadIdx.x] = sum(w, b, e);
+    const int most = min(teams, JOIN_TEAMS);
+    const int64_t each = ceil_div64(terms, most), b = team * each, e = b + each < terms ? b + each : terms;
+    if (team < most) share[threadIdx.x] = sum(w, b, e);
     __syncthreads();
     if (team == 0 && have) {
       float4 acc = share[tl];
-      for (int t = 1; t < teams; ++t) {
+#pragma unroll 4
+      for (int t = 1; t < most; ++t) {
         const float4 v = share[(t << a.log_l) + tl];
         acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
       }
@@ -1009,10 +1011,10 @@ __global__ __launch_bounds__(THREADS) void k_range_sort(small_args a, range_work
 constexpr int RANGE_RUNS = 64;        // runs whose places are looked up together
 template <int THREADS, class TI, class TO, int VEC>
 __global__ __launch_bounds__(THREADS) void k_range_sums(small_args a, range_work w, int ranges, int64_t* __restrict__ ids, int32_t* __restrict__ count) {
-  __shared__ uint32_t wave_sum[THREADS / 64], queue[64], row[MAX_RANGES + 1], first[MAX_RANGES + 1], begin[RANGE_RUNS + 1], key[RANGE_RUNS];
+  __shared__ uint32_t wave_sum[THREADS / 64], queue[64], row[MAX_RANGES + 1], first[MAX_RANGES + 1], begin[2 * RANGE_RUNS], key[RANGE_RUNS];
   __shared__ int queued;
   __shared__ float parts[THREADS * 8];
-  static_assert(MAX_RANGES <= THREADS, "a thread per range");
+  static_assert(MAX_RANGES <= THREADS && 2 * RANGE_RUNS <= THREADS, "a thread per range, and per end of a run");
   const int t = threadIdx.x, lane = t & 63;
   const uint32_t mine = t < ranges ? w.distinct[t] : 0u, inc = wave_inclusive(mine);
   if (t <= MAX_RANGES) first[t] = t <= ranges ? w.first[t] : 0u;
@@ -1025,27 +1027,30 @@ __global__ __launch_bounds__(THREADS) void k_range_sums(small_args a, range_work
   __syncthreads();
   if (blockIdx.x == 0 && t == 0) *count = (int32_t)all;
   const int share = (int)(gridDim.x / (uint32_t)a.col_blocks), sh = (int)(blockIdx.x / (uint32_t)a.col_blocks);
-  const int r1 = (int)((int64_t)all * (sh + 1) / share);
-  for (int r0 = (int)((int64_t)all * sh / share); r0 < r1; r0 += RANGE_RUNS) {
-    const int runs = min(RANGE_RUNS, r1 - r0);
-    if (t <= runs) {            // where run r0 + t begins; the last one's end is where the next one would
-      int k = 0;                // its range: row[k] <= r0 + t < row[k + 1]
+  // runs sh, sh + share, ..: frequent ids are often neighbours
+  const int mine_all = ((int)all - sh + share - 1) / share;
+  for (int r0 = 0; r0 < mine_all; r0 += RANGE_RUNS) {
+    const int runs = min(RANGE_RUNS, mine_all - r0);
+    if (t < 2 * runs) {         // where a run begins, and the one after it, which is its end
+      const int r = sh + (r0 + (t >> 1)) * share + (t & 1);
+      int k = 0;                // its range: row[k] <= r < row[k + 1]
 #pragma unroll
-      for (int step = MAX_RANGES / 2; step; step >>= 1) k += (int)row[k + step] <= r0 + t ? step : 0;
-      const bool none = (uint32_t)(r0 + t) >= all;
-      const uint32_t at = first[k] + (uint32_t)(r0 + t) - row[k];
+      for (int step = MAX_RANGES / 2; step; step >>= 1) k += (int)row[k + step] <= r ? step : 0;
+      const bool none = (uint32_t)r >= all;
+      const uint32_t at = first[k] + (uint32_t)r - row[k];
       begin[t] = none ? first[ranges] : first[k] + w.heads[at];
-      if (t < runs) key[t] = w.key[at];
+      if (!(t & 1)) key[t >> 1] = w.key[at];
     }
     __syncthreads();
     small_sums<THREADS, TI, VEC>(
-        a, runs, [&](int r) { return (int)begin[r]; }, [&](int r) { return (int)begin[r + 1]; }, [&](int k) { return w.pos[k]; },
+        a, runs, [&](int r) { return (int)begin[2 * r]; }, [&](int r) { return (int)begin[2 * r + 1]; }, [&](int k) { return w.pos[k]; },
         [&](int r, const float (&acc)[VEC], int col, int own) {
-          if (col == 0) ids[r0 + r] = (int64_t)key[r];
+          const int64_t to = sh + (int64_t)(r0 + r) * share;
+          if (col == 0) ids[to] = (int64_t)key[r];
           float f[VEC];
 #pragma unroll
           for (int j = 0; j < VEC; ++j) f[j] = acc[j] * a.scale;
-          store_chunk<VEC, TO>((TO*)a.out + (int64_t)(r0 + r) * a.ld_out + col, f);
+          store_chunk<VEC, TO>((TO*)a.out + to * a.ld_out + col, f);
         },
         parts, queue, &queued);
     __syncthreads();
@@ -1128,7 +1133,10 @@ int launch_sums(seg_args a, bool accumulate, hipStream_t stream) {
 }
 
 bool is_small(int64_t n, int64_t width) { return n <= SMALL_N && n * width <= SMALL_VALUES; }
-bool maps(int64_t num_rows) { return num_rows <= 256LL * SMALL_MAP; }        // the workgroups of k_small can mark that many rows
+// whether k_small's workgroups mark the rows and zero the others: as many rows as they can mark, and no more bytes than pay a launch of
+// its own (20 ids in rows of 256 bf16, marked and filled ahead: 16 MB 8.2 and 10.1 us, 64 MB 15.8 and 16.2, 128 MB 24.9 and 24.0, 256 MB 42.9
+// and 39.5)
+bool maps(int64_t num_rows, int64_t bytes) { return num_rows <= 256LL * SMALL_MAP && bytes <= 128 * MB; }
 template <class T> void columns(small_args* a) {
   constexpr int VEC = elems16<T>;
   a->chunks = a->width < VEC ? a->width : (a->width + VEC - 1) / VEC;
@@ -1192,9 +1200,10 @@ int small_rows(small_args a, char* ws, int64_t* ids, int32_t* count, hipStream_t
   const range_work w = range_layout(ws, a.n, &bytes);
   const int ranges = (int)std::min<int64_t>(MAX_RANGES, ceil_div64(a.n, 4));
   if (int rc = a.n <= TINY_N ? launch_range_sort<TINY_THREADS>(a, w, ranges, stream) : launch_range_sort<SMALL_THREADS>(a, w, ranges, stream)) return rc;
-  // a run per team and workgroup, at most 1024 teams' waves per CU (and a workgroup for each column block)
+  // a run per team, no more than are looked up at once, and at most a workgroup per CU (two small ones; one for each column block)
   const int threads = a.n <= TINY_N ? TINY_THREADS : SMALL_THREADS;
-  const int64_t shares = std::max<int64_t>(1, std::min(ceil_div64(a.n, threads >> a.log_l), ceil_div64(a.n <= TINY_N ? 512 : 256, a.col_blocks)));
+  const int64_t runs = std::min(RANGE_RUNS, threads >> a.log_l);
+  const int64_t shares = std::max<int64_t>(1, std::min(ceil_div64(a.n, runs), ceil_div64(a.n <= TINY_N ? 512 : 256, a.col_blocks)));
   const unsigned grid = (unsigned)(shares * a.col_blocks);
   auto* kernel = a.n <= TINY_N ? (a.width >= VEC ? k_range_sums<TINY_THREADS, TI, TO, VEC> : k_range_sums<TINY_THREADS, TI, TO, 1>)
                                : (a.width >= VEC ? k_range_sums<SMALL_THREADS, TI, TO, VEC> : k_range_sums<SMALL_THREADS, TI, TO, 1>);
@@ -1214,7 +1223,7 @@ int64_t workspace_bytes_of(int64_t n, int64_t width, int64_t num_rows) {
   if (!is_small(n, width)) return layout(n, width, num_rows).bytes;
   int64_t bytes;
   range_layout(nullptr, n, &bytes);
-  return maps(num_rows) ? bytes : std::max(bytes, layout(n, width, num_rows).bytes);
+  return bytes;
 }
 
 int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, const int64_t* idx64, const int32_t* idx32, int64_t n, int64_t width,
@@ -1232,11 +1241,18 @@ int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, co
   return ORCA_OK;
 }
 
-// the pieces of a fill that launch `i` of `launches` takes, and the workgroups for them
+// the pieces of a fill that launch `i` of `launches` takes, and the workgroups for them.  (Even shares: a million rows of 400 bytes 84 us;
+// 24 and 40 MB in the sort's launches, what they need in time, and the rest in k_fill: 90; everything in the first launch: 105.)
 unsigned fill_share(fill_job* f, int64_t pieces, int i, int launches) {
   f->from = pieces * i / launches;
   f->to = pieces * (i + 1) / launches;
-  return (unsigned)std::min<int64_t>(f->to - f->from, 4096);
+  return (unsigned)std::min<int64_t>(f->to - f->from, 1 << 20);
+}
+int launch_fill(fill_job f, int64_t pieces, hipStream_t stream) {
+  const unsigned blocks = fill_share(&f, pieces, 0, 1);
+  if (blocks) k_fill<<<blocks, 1024, 0, stream>>>(f);
+  ORCA_LAUNCH_CHECK();
+  return ORCA_OK;
 }
 
 // sorts (id, position), zeroes the fill's pieces on the way; *sorted = where the result lies
@@ -1305,13 +1321,14 @@ ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64
     pieces = (gaps ? num_rows : 1) * fill.per_row;
     fill.past = past_zeros(num_rows * width * e);
   }
-  if (n == 0) {
-    if (pieces) k_fill<<<fill_share(&fill, pieces, 0, 1), 512, 0, stream>>>(fill);
-    ORCA_LAUNCH_CHECK();
-    return ORCA_OK;
-  }
-  if (is_small(n, width) && (accumulate || maps(num_rows))) {
-    const small_args a{idx64, idx32, num_rows, padding_idx, grad_out, ld_grad, ld_table, grad_table, (int)n, (int)width, 0, 0, 0, !accumulate, scale};
+  if (n == 0) return launch_fill(fill, pieces, stream);
+  // (the order of the sum's launch and the fill's: a tall table is filled first, as a whole and faster)
+  const bool marks = !accumulate && maps(num_rows, num_rows * width * (table_dtype == ORCA_F32 ? 4 : 2));
+  if (is_small(n, width)) {
+    if (!accumulate && !marks) {
+      if (int rc = launch_fill(fill, pieces, stream)) return rc;
+    }
+    const small_args a{idx64, idx32, num_rows, padding_idx, grad_out, ld_grad, ld_table, grad_table, (int)n, (int)width, 0, 0, 0, marks, scale};
     return by_types(grad_dtype, table_dtype, [&](auto gi, auto go) {
       return n <= TINY_N ? small_dense<TINY_THREADS, decltype(gi), decltype(go)>(a, accumulate != 0, stream)
                          : small_dense<SMALL_THREADS, decltype(gi), decltype(go)>(a, accumulate != 0, stream);
