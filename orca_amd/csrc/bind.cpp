@@ -6,6 +6,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <algorithm>
@@ -74,6 +75,12 @@ void arguments(Py_ssize_t n, Py_ssize_t want) {
   if (n != want) refuse(PyExc_TypeError, "expected ", want, " arguments, got ", n);
 }
 
+// an output that shares memory with an input
+void apart(const at::Tensor& out, const at::Tensor& in, const char* who, const char* what) {
+  const at::MemOverlapStatus s = at::get_overlap_status(out, in);
+  if (s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial) refuse(PyExc_ValueError, who, ": out overlaps ", what);
+}
+
 // embedding(table, ids, scale, out)
 PyObject* embedding(PyObject* const* a, Py_ssize_t n) {
   arguments(n, 4);
@@ -97,6 +104,7 @@ PyObject* embedding(PyObject* const* a, Py_ssize_t n) {
     out = elements(a[3], "embedding out", &c);
     if (c != code || out.device() != dev || !out.is_contiguous() || out.sizes() != at::IntArrayRef(shape))
       refuse(PyExc_ValueError, "embedding: out must be a contiguous ", table.scalar_type(), " tensor of shape ", at::IntArrayRef(shape), " on ", dev);
+    apart(out, table, "embedding", "the table");
   }
   check(embedding_forward(table.const_data_ptr(), code, table.size(0), width, table.stride(0), ids.i64, ids.i32, ids.t.numel(), (float)scale,
                           out.data_ptr(), stream_of(dev)),
@@ -166,6 +174,7 @@ PyObject* embedding_backward(PyObject* const* a, Py_ssize_t n) {
         (b.num_rows > 1 && out.stride(0) < b.width) || (type != b.code && type != ORCA_F32) || (a[7] != Py_None && type_of(a[7], b, who) != type))
       refuse(PyExc_ValueError, "embedding_backward: out must be a tensor of shape [", b.num_rows, ", ", b.width, "] on ", b.dev,
              " of the gradient's type or float32, whose rows are contiguous and do not overlap");
+    apart(out, b.g, who, "grad_out");
   }
   check(embedding_backward_c(b.g.const_data_ptr(), b.code, b.n ? b.g.stride(0) : 0, b.ids.i64, b.ids.i32, b.n, b.width, b.num_rows, b.padding, b.scale,
                              accumulate, out.data_ptr(), type, out.stride(0), ws.data_ptr(), bytes, stream_of(b.dev)),
@@ -201,6 +210,8 @@ PyObject* embedding_backward_rows(PyObject* const* a, Py_ssize_t n) {
         (a[6] != Py_None && type_of(a[6], b, who) != type))
       refuse(PyExc_ValueError, who, ": out must be contiguous int64 [", b.n, "], gradient-typed or float32 [", b.n, ", ", b.width,
              "] and int32 [1] tensors on ", b.dev);
+    apart(rows, b.g, who, "grad_out");
+    apart(ids, b.ids.t, who, "the ids");
   }
   check(embedding_backward_rows_c(b.g.const_data_ptr(), b.code, b.n ? b.g.stride(0) : 0, b.ids.i64, b.ids.i32, b.n, b.width, b.num_rows, b.padding,
                                   b.scale, (int64_t*)ids.data_ptr(), rows.data_ptr(), type, (int32_t*)count.data_ptr(), ws.data_ptr(), bytes,
@@ -293,6 +304,22 @@ PyObject* grad_norm(PyObject* const* a, Py_ssize_t n) {
   return r;
 }
 
+// the bytes of the list's tensors: where they begin, where they end
+typedef std::pair<const char*, const char*> span;
+span span_of(const void* p, int64_t n, int code) { return {(const char*)p, (const char*)p + n * (code == ORCA_F32 ? 4 : 2)}; }
+std::vector<span> spans_of(const grad_arrays& g) {
+  std::vector<span> s;
+  s.reserve(g.data.size());
+  for (size_t i = 0; i < g.data.size(); ++i)
+    if (g.sizes[i]) s.push_back(span_of(g.data[i], g.sizes[i], g.types[i]));
+  return s;
+}
+void apart_in_list(std::vector<span> s, const char* who) {
+  std::sort(s.begin(), s.end());
+  for (size_t i = 1; i < s.size(); ++i)
+    if (s[i].first < s[i - 1].second) refuse(PyExc_ValueError, who, ": a tensor is in the list twice, or two of them overlap");
+}
+
 // clip_grad_norm(list, max_norm, flat buffers or None) -> norm
 PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
   arguments(n, 3);
@@ -302,11 +329,7 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
   const c10::DeviceGuard guard(g.dev);
   void* flat[3] = {nullptr, nullptr, nullptr};
   if (a[2] == Py_None) {
-    std::vector<void*> seen;
-    for (size_t i = 0; i < g.data.size(); ++i)
-      if (g.sizes[i]) seen.push_back(g.data[i]);
-    std::sort(seen.begin(), seen.end());
-    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) refuse(PyExc_ValueError, who, ": a gradient is in the list twice");
+    apart_in_list(spans_of(g), who);
     for (const auto& c : g.copies)
       for (int64_t d = 0; d < c.second.dim(); ++d)
         if (c.second.stride(d) == 0 && c.second.size(d) > 1) refuse(PyExc_ValueError, who, ": an expanded tensor cannot be clipped in place");
@@ -314,6 +337,7 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
     if (!PyList_Check(a[2])) refuse(PyExc_TypeError, who, ": flat must be a list of tensors");
     std::vector<int> order;                       // the types as they first appear
     int64_t need[3] = {0, 0, 0};
+    std::vector<span> written;
     for (size_t i = 0; i < g.data.size(); ++i) {
       const int t = g.types[i];
       if (std::find(order.begin(), order.end(), t) == order.end()) order.push_back(t);
@@ -327,7 +351,14 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
       if (code != order[k] || f.numel() != need[code] || f.device() != g.dev || !f.is_contiguous())
         refuse(PyExc_ValueError, who, ": flat buffer ", k, " is not a contiguous ", TYPES[order[k]], " tensor of ", need[order[k]], " elements on ", g.dev);
       flat[code] = f.data_ptr();
+      if (f.numel()) written.push_back(span_of(f.data_ptr(), f.numel(), code));
     }
+    for (size_t i = 0; i < g.data.size(); ++i) {
+      const span r = span_of(g.data[i], g.sizes[i], g.types[i]);
+      for (const span& w : written)
+        if (w.first < r.second && r.first < w.second) refuse(PyExc_ValueError, who, ": a flat buffer overlaps a gradient");
+    }
+    apart_in_list(std::move(written), who);
   }
   const auto opt = at::TensorOptions(g.dev).dtype(at::kFloat);
   const at::Tensor norm = at::empty({}, opt), ws = at::empty({grad_norm_workspace_bytes()}, opt.dtype(at::kByte));

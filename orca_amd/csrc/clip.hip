@@ -216,6 +216,7 @@ int64_t bytes_of(const host_list& h, int i) { return h.sizes[i] * (h.dtypes[i] =
 int check_list(const char* who, host_list* h, double max_norm, const float* norm, const void* workspace) {
   ORCA_REQUIRE(h->n >= 0 && h->n <= 65536 && norm && workspace && (h->n == 0 || (h->grads && h->sizes && h->dtypes)) && (!h->rows || h->widths),
                "%s: null argument, or not 0 to 65536 tensors", who);
+  ORCA_REQUIRE(((uintptr_t)workspace & 7) == 0, "%s: the workspace is not 8-byte aligned", who);
   ORCA_REQUIRE(max_norm >= 0.0, "%s: max_norm %g (not negative, not NaN)", who, max_norm);
   int64_t total = 0;
   for (int i = 0; i < h->n; ++i) {

@@ -1236,6 +1236,7 @@ int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, co
   if (n == 0) return ORCA_OK;
   ORCA_REQUIRE(g && (idx64 != nullptr) != (idx32 != nullptr), "%s: null gradient, or not exactly one list of ids", who);
   ORCA_REQUIRE(ld_g >= 0, "%s: negative row stride", who);
+  ORCA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: the workspace is not 16-byte aligned", who);
   ORCA_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(n, width, num_rows), "%s: the workspace holds %lld of %lld bytes", who,
                (long long)workspace_bytes, (long long)workspace_bytes_of(n, width, num_rows));
   return ORCA_OK;

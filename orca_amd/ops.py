@@ -615,7 +615,7 @@ def _load_host():
 def embedding(table, ids, scale=1.0, out=None):
   """orca_embedding_forward: scale * table[ids] -- table [n_rows, width] fp32 / bf16 / fp16 (rows may be strided), ids int64 or
   int32 of any shape -> [*ids.shape, width] in the table's type (fp32 product, one rounding).  An id outside the table reads as
-  zeros.  out: a contiguous tensor of that shape and type.  No autograd: torch.ops.orca.embedding has it."""
+  zeros.  out: a contiguous tensor of that shape and type, apart from the table.  No autograd: torch.ops.orca.embedding has it."""
   return (_host or _load_host()).embedding(table, ids, scale, out)
 
 
@@ -681,7 +681,9 @@ class FusedAdam:
       if g is None:
         continue
       if isinstance(g, RowGrad):
-        if p.dim() != 2 or g.rows.shape[1:] != p.shape[1:] or g.num_rows != p.shape[0] or g.rows.dtype != torch.float32 or not g.rows.is_cuda:
+        if (p.dim() != 2 or g.rows.dim() != 2 or g.rows.shape[1] != p.shape[1] or g.num_rows != p.shape[0] or g.ids.shape != g.rows.shape[:1]
+            or g.count.numel() != 1 or (g.ids.dtype, g.rows.dtype, g.count.dtype) != (torch.int64, torch.float32, torch.int32)
+            or any(t.device != p.device or not t.is_contiguous() for t in (g.ids, g.rows, g.count))):
           raise _lib.OrcaError(f"FusedAdam: row gradient of {k} does not match its parameter")
         used[k] = g
       else:

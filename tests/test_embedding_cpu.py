@@ -127,3 +127,10 @@ def test_adam_rows_refusals():
     refused(rows(**{bad: None}), "null argument")
   assert rows(room=0, ids=None) == 0
   refused(_lib.load().orca_adam_step_scaled(1, None, None, None, None, None, 1e-3, 0.9, 0.999, 1e-8, 1, None, None), "bad arguments")
+
+
+def test_unaligned_workspaces():
+  for rows in (False, True):
+    refused(backward(rows, ws=P + 8), "aligned")
+  for norm_only in (False, True):
+    refused(clip(ws=P + 4, norm_only=norm_only), "aligned")

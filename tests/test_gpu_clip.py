@@ -241,3 +241,30 @@ def test_refusals(ops):
   with pytest.raises(ValueError):
     ops.clip_grad_norm([g], 1.0, flat=[])
   assert bool((g == 1).all())
+
+
+def test_overlaps_are_refused(ops):
+  buf = torch.ones(100, device=DEV)
+  with pytest.raises(ValueError, match="overlap"):
+    ops.clip_grad_norm([buf[:50], buf[49:]], 1.0)
+  with pytest.raises(ValueError, match="overlap"):
+    ops.clip_grad_norm([buf[:50]], 1.0, flat=[buf[40:90]])
+  with pytest.raises(ValueError, match="overlap"):
+    ops.clip_grad_norm([buf[:10], torch.ones(4, device=DEV, dtype=torch.float16)], 1.0, flat=[buf[20:30], buf.view(torch.float16)[58:62]])
+  assert bool((buf == 1).all())
+  # neighbours: 20 squares of 1
+  norm = ops.clip_grad_norm([buf[:10], buf[10:20]], 1e-3, flat=[buf[20:40]])
+  assert abs(float(norm) - 20 ** 0.5) <= 20 ** 0.5 * 2 * U and bool((buf[:20] == 1).all()) and bool((buf[20:40] < 1).all()) and bool((buf[40:] == 1).all())
+
+
+def test_on_another_stream(ops):
+  s = torch.cuda.Stream()
+  grads = make([100, 300000], TYPES[:1], seed=4)
+  want = [x.clone() for x in grads]
+  n0 = ops.clip_grad_norm(want, 0.5)
+  torch.cuda.synchronize()
+  with torch.cuda.stream(s):
+    got = [x * 1.0 for x in grads]
+    n1 = ops.clip_grad_norm(got, 0.5)
+  s.synchronize()
+  assert torch.equal(n0, n1) and all(torch.equal(a, b) for a, b in zip(got, want))

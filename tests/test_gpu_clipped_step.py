@@ -205,3 +205,20 @@ def test_refusals(ops):
   with pytest.raises(ValueError):
     opt.step({"t": torch.zeros(10, 4, device=DEV)}, max_norm=-1.0)
   assert opt.steps["t"] == 0
+
+
+def test_row_gradients_that_do_not_fit(ops):
+  """a RowGrad made by hand: fewer rows than ids, other types, gaps, another device"""
+  from orca_amd._lib import OrcaError
+  opt = ops.FusedAdam({"t": torch.zeros(10, 4, device=DEV)}, lr=1e-2)
+  ids, rows, cnt = torch.arange(3, device=DEV), torch.ones(3, 4, device=DEV), torch.full((1,), 3, dtype=torch.int32, device=DEV)
+  for bad in (ops.RowGrad(ids, rows[:2], cnt, 10), ops.RowGrad(ids.int(), rows, cnt, 10), ops.RowGrad(ids, rows, cnt.long(), 10),
+              ops.RowGrad(ids, torch.ones(3, 8, device=DEV)[:, ::2], cnt, 10), ops.RowGrad(torch.arange(6, device=DEV)[::2], rows, cnt, 10),
+              ops.RowGrad(ids.cpu(), rows, cnt, 10), ops.RowGrad(ids, rows, cnt.cpu(), 10), ops.RowGrad(ids, rows, cnt.repeat(2), 10),
+              ops.RowGrad(ids, rows.reshape(12), cnt, 10)):
+    for max_norm in (None, 1.0):
+      with pytest.raises(OrcaError):
+        opt.step({"t": bad}, max_norm=max_norm)
+  assert opt.steps["t"] == 0 and bool((opt.params["t"] == 0).all())
+  opt.step({"t": ops.RowGrad(ids, rows, cnt, 10)})
+  assert bool((opt.params["t"][:3] != 0).all()) and bool((opt.params["t"][3:] == 0).all())

@@ -402,3 +402,90 @@ def test_refusals_on_the_device(ops):
     ops.embedding_backward_rows(g, ids, 1 << 31)
   with pytest.raises(ValueError):
     ops.embedding_backward_rows(g, ids, 5, out=(ids, g, torch.zeros(1, device=DEV)))
+
+
+def test_outputs_apart_from_inputs(ops):
+  """an output that shares memory with what the call reads is refused; neighbours in one buffer are not"""
+  buf = torch.randn(20, 8, device=DEV)
+  ids = torch.tensor([1, 0, 3], device=DEV)
+  for out in (buf[:3], buf[2:5]):
+    with pytest.raises(ValueError, match="overlaps"):
+      ops.embedding(buf[:4], ids, out=out)
+  with pytest.raises(ValueError, match="overlaps"):
+    ops.embedding_backward(buf[:3], ids, 5, out=buf[2:7])
+  with pytest.raises(ValueError, match="overlaps"):
+    ops.embedding_backward_rows(buf[:3], ids, 5, out=(torch.zeros(3, dtype=torch.int64, device=DEV), buf[1:4], torch.zeros(1, dtype=torch.int32, device=DEV)))
+  with pytest.raises(ValueError, match="overlaps"):
+    ops.embedding_backward_rows(buf[:3], ids, 5, out=(ids, torch.zeros(3, 8, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)))
+  want = buf[:4][ids].clone()
+  assert torch.equal(ops.embedding(buf[:4], ids, out=buf[4:7]), want)
+  before = buf[:4].clone()
+  got = ops.embedding_backward(buf[:3], ids, 5, out=buf[10:15])
+  check_grad(got, before[:3], ids, 5, 1.0, None)
+  assert torch.equal(buf[:4], before)
+
+
+def test_long_lists_captured_and_replayed(ops):
+  """the sort's launches in a graph, other contents and eager work between the replays"""
+  n, vocab, w = 12000, 5000, 20
+  ids, grad = torch.zeros(n, dtype=torch.int32, device=DEV), torch.zeros(n, w, device=DEV, dtype=torch.bfloat16)
+
+  def step():
+    return ops.embedding_backward(grad, ids, vocab, 2.0, dtype=torch.float32), ops.embedding_backward_rows(grad, ids, vocab)
+
+  step()
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    dense, rg = step()
+  for r, kind in enumerate(["uniform", "same", "hubs"]):
+    ids.copy_(make_ids(kind, n, vocab, r).clamp_(max=vocab - 1))
+    grad.copy_(torch.randn(n, w, generator=torch.Generator().manual_seed(r)))
+    graph.replay()
+    torch.cuda.synchronize()
+    e_dense, e_rg = step()
+    k = int(e_rg.count)
+    assert torch.equal(dense, e_dense), f"replay {r}"
+    assert int(rg.count) == k and torch.equal(rg.ids[:k], e_rg.ids[:k]) and torch.equal(rg.rows[:k], e_rg.rows[:k]), f"replay {r}"
+
+
+def test_autograd_on_another_stream(ops):
+  """forward under a stream: the backward pass runs on it, behind what the gradient's producer left there"""
+  from orca_amd import torch_ops  # noqa: F401
+  vocab, w, n = 3000, 64, 20000
+  g = torch.Generator().manual_seed(8)
+  table = torch.randn(vocab, w, generator=g).to(DEV).requires_grad_()
+  ids, wgt = torch.randint(0, vocab, (n,), generator=g).to(DEV), torch.randn(n, w, generator=g).to(DEV)
+  torch.cuda.synchronize()
+  s = torch.cuda.Stream()
+  with torch.cuda.stream(s):
+    grad, = torch.autograd.grad((torch.ops.orca.embedding(table, ids, 1.0, -1) * wgt).sum(), table)
+  s.synchronize()
+  check_grad(grad, wgt, ids, vocab, 1.0, None)
+
+
+def test_neighbouring_hubs_row_sparse(ops):
+  """frequent ids side by side (each longer than a team adds alone), among rare ones, over widths with few and many teams"""
+  for n, w, seed in ((700, 2, 0), (2048, 40, 1), (2049, 3, 2), (6000, 100, 3), (8192, 16, 4), (8192, 128, 5), (1024, 1024, 6)):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.where(torch.rand(n, generator=g) < 0.8, torch.randint(500, 508, (n,), generator=g), torch.randint(0, 4000, (n,), generator=g)).to(DEV)
+    grad = torch.randn(n, w, generator=g).to(DEV)
+    rg = ops.embedding_backward_rows(grad, ids, 4000)
+    k = int(rg.count)
+    assert torch.equal(rg.ids[:k], torch.unique(ids))
+    check_grad(torch.zeros(4000, w, device=DEV).index_copy_(0, rg.ids[:k], rg.rows[:k]), grad, ids, 4000, 1.0, None)
+
+
+def test_tables_of_all_heights_behind_short_lists(ops):
+  """both ways to the zeros: marked rows in the sum's launch, and a fill ahead of it (from 128 MB on, or 16.8 million rows)"""
+  for vocab, w, t in ((250000, 128, torch.bfloat16), (250001, 160, torch.float32), (16777217, 2, torch.bfloat16), (16777216, 1, torch.float32)):
+    ids = torch.tensor([0, vocab - 1, 7, 7, vocab, -1, vocab // 2], device=DEV)
+    grad = torch.randn(7, w, device=DEV).to(t)
+    out = torch.full((vocab, w), 3.0, dtype=t, device=DEV)
+    got = ops.embedding_backward(grad, ids, vocab, out=out)
+    rows = torch.tensor([0, 7, vocab // 2, vocab - 1], device=DEV)
+    assert int((got != 0).any(1).sum()) == 4
+    exp = torch.stack([grad[0].double(), grad[2].double() + grad[3].double(), grad[6].double(), grad[1].double()])
+    # one fp32 sum of two (half a step of 2^-24) and one rounding to the type
+    lim = exp.abs() * (2.0 ** -24 + torch.finfo(t).eps / 2) * 1.01 + 1e-30
+    assert bool(((got[rows].double() - exp).abs() <= lim).all())
