@@ -109,27 +109,25 @@ int embedding_typed(const void* table, int64_t n_rows, int64_t width, int64_t ld
 // ---- zeros ahead of the sums -----------------------------------------------------------------------------------------
 // A dense gradient starts as zeros; nothing before the sums reads it, so the launches of the sort carry the zero fill in extra
 // workgroups: the sort waits on latency with a few dozen workgroups, the fill on the HBM, and the longer of the two is what counts.
-constexpr int FILL_PIECE = 16384;       // bytes a workgroup writes: few and in order (400 MB in pieces of 32 KB 74 us, of 16 KB, a store per thread 60)
+// A piece is one 16-byte store for each of 256 threads: 640 MB in workgroups of 256 threads 94 us, 512 100, 1024 104, several stores a
+// thread 105 to 107, a grid of 2048 that goes round 118.
+constexpr int FILL_PIECE = 4096;
 struct fill_job {
-  char* p;                      // `rows` rows of `bytes` bytes, `pitch` bytes apart (a table without gaps is one row)
+  char* p;                      // `rows` rows of `bytes` bytes, `pitch` bytes apart (a table without gaps is one row, pitch 0)
   int64_t bytes, pitch, per_row, from, to;      // pieces of a row; this launch's pieces
   int past;
 };
 template <int THREADS, bool PAST> __device__ __forceinline__ void fill_loop(const fill_job& f, int64_t block, int64_t blocks) {
   const u32x4 zero = {0, 0, 0, 0};
-  for (int64_t i = f.from + block; i < f.to; i += blocks) {
-    const int64_t r = i / f.per_row, at = (i - r * f.per_row) * FILL_PIECE;
+  for (int64_t i = f.from + block * (THREADS / 256) + (threadIdx.x >> 8); i < f.to; i += blocks * (THREADS / 256)) {
+    const int64_t r = f.pitch ? i / f.per_row : 0, at = (i - r * f.per_row) * FILL_PIECE;
     char* p = f.p + r * f.pitch + at;
-    const int len = (int)(f.bytes - at < FILL_PIECE ? f.bytes - at : FILL_PIECE);
-#pragma unroll
-    for (int k = 0; k < FILL_PIECE / (16 * THREADS); ++k) {
-      const int b = ((int)threadIdx.x + THREADS * k) * 16;
-      if (b + 16 <= len) {
-        if constexpr (PAST) store16_past(p + b, zero);
-        else store16(p + b, zero);
-      } else {
-        for (int e = b; e < len; e += 2) *reinterpret_cast<uint16_t*>(p + e) = 0;
-      }
+    const int len = (int)(f.bytes - at < FILL_PIECE ? f.bytes - at : FILL_PIECE), b = (int)(threadIdx.x & 255) * 16;
+    if (b + 16 <= len) {
+      if constexpr (PAST) store16_past(p + b, zero);
+      else store16(p + b, zero);
+    } else {
+      for (int e = b; e < len; e += 2) *reinterpret_cast<uint16_t*>(p + e) = 0;
     }
   }
 }
@@ -137,7 +135,7 @@ template <int THREADS> __device__ __forceinline__ void fill_pieces(const fill_jo
   if (f.past) fill_loop<THREADS, true>(f, block, blocks);
   else fill_loop<THREADS, false>(f, block, blocks);
 }
-__global__ __launch_bounds__(1024) void k_fill(fill_job f) { fill_pieces<1024>(f, blockIdx.x, gridDim.x); }
+__global__ __launch_bounds__(256) void k_fill(fill_job f) { fill_pieces<256>(f, blockIdx.x, gridDim.x); }
 
 // ---- sort of the positions by id -------------------------------------------------------------------------------------
 // Stable least-significant-digit radix sort of (key, position) pairs; key = the id, or num_rows for what has no row (the padding
@@ -1133,10 +1131,11 @@ int launch_sums(seg_args a, bool accumulate, hipStream_t stream) {
 }
 
 bool is_small(int64_t n, int64_t width) { return n <= SMALL_N && n * width <= SMALL_VALUES; }
-// whether k_small's workgroups mark the rows and zero the others: as many rows as they can mark, and no more bytes than pay a launch of
-// its own (20 ids in rows of 256 bf16, marked and filled ahead: 16 MB 8.2 and 10.1 us, 64 MB 15.8 and 16.2, 128 MB 24.9 and 24.0, 256 MB 42.9
-// and 39.5)
-bool maps(int64_t num_rows, int64_t bytes) { return num_rows <= 256LL * SMALL_MAP && bytes <= 128 * MB; }
+// Whether k_small's workgroups mark the rows and zero the others: as many rows as they can mark, and no more bytes than pay a launch of
+// its own, whose stores run at the full rate.  Marked and filled ahead, us, workgroups of 256 threads (20 ids in rows of 49 fp32): 16 MB 9.0
+// and 8.5, 24 MB 10.9 and 9.3, 64 MB 19.6 and 14.3 (rows of 256 bf16: 8.2 and 8.7, 9.6 and 9.8, 15.9 and 14.3); of 1024 threads (2500 ids in
+// rows of 8 fp32): 24 MB 15.0 and 16.7, 64 MB 20.4 and 22.4, 128 MB 27.6 and 30.1, 160 MB 33.4 and 33.8.
+bool maps(int64_t n, int64_t num_rows, int64_t bytes) { return num_rows <= 256LL * SMALL_MAP && bytes <= (n <= TINY_N ? 20 : 160) * MB; }
 template <class T> void columns(small_args* a) {
   constexpr int VEC = elems16<T>;
   a->chunks = a->width < VEC ? a->width : (a->width + VEC - 1) / VEC;
@@ -1242,16 +1241,16 @@ int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, co
   return ORCA_OK;
 }
 
-// the pieces of a fill that launch `i` of `launches` takes, and the workgroups for them.  (Even shares: a million rows of 400 bytes 84 us;
-// 24 and 40 MB in the sort's launches, what they need in time, and the rest in k_fill: 90; everything in the first launch: 105.)
-unsigned fill_share(fill_job* f, int64_t pieces, int i, int launches) {
+// the pieces of a fill that launch `i` of `launches` takes, and the workgroups for them.  (Even shares: a million rows of 400 bytes 81 us;
+// 80 MB in the sort's launches and the rest ahead of the sums: 92; everything ahead of the sort: 100.)
+unsigned fill_share(fill_job* f, int64_t pieces, int threads, int i, int launches) {
   f->from = pieces * i / launches;
   f->to = pieces * (i + 1) / launches;
-  return (unsigned)std::min<int64_t>(f->to - f->from, 1 << 20);
+  return (unsigned)std::min<int64_t>(ceil_div64(f->to - f->from, threads / 256), 1 << 24);
 }
 int launch_fill(fill_job f, int64_t pieces, hipStream_t stream) {
-  const unsigned blocks = fill_share(&f, pieces, 0, 1);
-  if (blocks) k_fill<<<blocks, 1024, 0, stream>>>(f);
+  const unsigned blocks = fill_share(&f, pieces, 256, 0, 1);
+  if (blocks) k_fill<<<blocks, 256, 0, stream>>>(f);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
@@ -1265,14 +1264,14 @@ int sort_positions(const int64_t* idx64, const int32_t* idx32, int64_t n, int64_
   uint32_t* totals = s.tiles > DIRECT_TILES ? (uint32_t*)(ws + l.totals) : nullptr;
   pair32* buf[2] = {(pair32*)(ws + l.a), (pair32*)(ws + l.b)};
   for (int p = 0; p < s.passes; ++p) {
-    unsigned extra = fill_share(&fill, pieces, 2 * p, 2 * s.passes);
+    unsigned extra = fill_share(&fill, pieces, SORT_THREADS, 2 * p, 2 * s.passes);
     k_sort_count<<<(unsigned)s.tiles + extra, SORT_THREADS, 0, stream>>>(src, p * s.digit, 1 << s.digit, counts, (int)s.tiles, fill);
     ORCA_LAUNCH_CHECK();
     if (totals) {
       k_sort_columns<<<((1 << s.digit) + 63) / 64, 64, 0, stream>>>(counts, s.tiles, 1 << s.digit, totals);
       ORCA_LAUNCH_CHECK();
     }
-    extra = fill_share(&fill, pieces, 2 * p + 1, 2 * s.passes);
+    extra = fill_share(&fill, pieces, SORT_THREADS, 2 * p + 1, 2 * s.passes);
     k_sort_scatter<<<(unsigned)s.tiles + extra, SORT_THREADS, 0, stream>>>(src, p * s.digit, s.digit, counts, totals, buf[p & 1], (int)s.tiles, fill);
     ORCA_LAUNCH_CHECK();
     src.pairs = buf[p & 1];
@@ -1317,14 +1316,13 @@ ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64
     const bool gaps = ld_table != width && num_rows > 1;
     fill.p = (char*)grad_table;
     fill.bytes = (gaps ? width : num_rows * width) * e;
-    fill.pitch = ld_table * e;
+    fill.pitch = gaps ? ld_table * e : 0;
     fill.per_row = ceil_div64(fill.bytes, FILL_PIECE);
     pieces = (gaps ? num_rows : 1) * fill.per_row;
     fill.past = past_zeros(num_rows * width * e);
   }
   if (n == 0) return launch_fill(fill, pieces, stream);
-  // (the order of the sum's launch and the fill's: a tall table is filled first, as a whole and faster)
-  const bool marks = !accumulate && maps(num_rows, num_rows * width * (table_dtype == ORCA_F32 ? 4 : 2));
+  const bool marks = !accumulate && maps(n, num_rows, num_rows * width * (table_dtype == ORCA_F32 ? 4 : 2));
   if (is_small(n, width)) {
     if (!accumulate && !marks) {
       if (int rc = launch_fill(fill, pieces, stream)) return rc;

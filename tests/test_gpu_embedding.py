@@ -489,3 +489,19 @@ def test_tables_of_all_heights_behind_short_lists(ops):
     # one fp32 sum of two (half a step of 2^-24) and one rounding to the type
     lim = exp.abs() * (2.0 ** -24 + torch.finfo(t).eps / 2) * 1.01 + 1e-30
     assert bool(((got[rows].double() - exp).abs() <= lim).all())
+
+
+def test_zeros_of_strided_tables(ops):
+  """a fill that leaves the gaps alone: rows of one piece and of several, by the sort's launches, ahead of a short list and alone"""
+  for n, vocab, w, ld, t in ((0, 300, 1500, 1501, torch.float32), (0, 5000, 3, 7, torch.bfloat16), (9000, 300, 2049, 2056, torch.float32),
+                             (9000, 4000, 5, 6, torch.float16), (3, 6000, 1100, 1111, torch.float32), (3, 1 << 20, 3, 16, torch.float32)):
+    g = torch.Generator().manual_seed(n + w)
+    ids = torch.randint(0, vocab, (n,), generator=g).to(DEV)
+    grad = torch.randn(n, w, generator=g).to(t).to(DEV)
+    buf = torch.full((vocab, ld), 5.0, dtype=t, device=DEV)
+    ops.embedding_backward(grad, ids, vocab, out=buf[:, :w])
+    assert bool((buf[:, w:] == 5).all())
+    if n > 100:
+      check_grad(buf[:, :w], grad, ids, vocab, 1.0, None)
+    else:
+      assert int((buf[:, :w] != 0).any(1).sum()) == torch.unique(ids).numel()
