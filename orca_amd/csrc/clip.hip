@@ -1,7 +1,8 @@
 // The global 2-norm of a list of gradient tensors and their scaling to a largest norm (torch.nn.utils.clip_grad_norm_'s formula):
 //   N = sqrt(sum g^2),  c = min(1, max_norm / (N + 1e-6)),  g <- c * g
-// Two launches per list, no atomics and no host read: k_norm_partial leaves one fp64 sum per workgroup, and every workgroup of k_clip
-// adds those sums up in the same order (while its first piece is on its way) before it scales its share.  Squares and sums are fp64:
+// No atomics and no host read.  Short lists, two launches: k_norm_partial leaves one fp64 sum per workgroup, and every workgroup of k_clip
+// adds those sums up in the same order (while its first piece is on its way) before it scales its share.  Long ones, where that time
+// shows: k_norm_finish adds them up in between, and a workgroup of k_clip takes a piece or four and ends.  Squares and sums are fp64:
 // neither overflows nor vanishes for any fp32 input, and the conversions hide behind the loads (4.5 elements per clock and CU at the
 // HBM rate for 16-bit gradients).
 //   A list travels in the kernel's arguments, under 4 KB: 12 bytes per tensor (16 with flat buffers), so that a few hundred tensors
@@ -10,11 +11,20 @@
 #include "elem.h"
 
 namespace {
-constexpr int PIECE = 16384, SMALL_PIECE = 4096;        // bytes a workgroup takes at a time: short lists spread over more workgroups
-// Flat buffers from here on: gradients read and products written past the caches (non-temporal).  Both ways measured, fp32 list, us:
-// 60 MB 33.1 against 31.6 with plain accesses, 120 MB 59.7 (71.9), 300 MB 142 (174), 1 GB 484 (552).
-constexpr int64_t STREAM_BYTES = 100000000;
-constexpr int PARTS = 2048;           // most partial sums of a call
+// Bytes a workgroup takes at a time: small pieces spread a short list over more workgroups.
+constexpr int PIECE = 16384, SMALL_PIECE = 4096, LONG_PIECE = 8192;
+// From here on a list is long, us for fp32 and both ways: into flat buffers 80 MB 41.0 (long: 45.6), 100 MB 54.9 (54.5), 120 MB 72.0 (63.2),
+// 500 MB 286 (246); in place 120 MB 55.6 (62.9), 160 MB 80.9 (80.1), 240 MB 133 (115), 1 GB 545 (466).
+constexpr int64_t LONG_FLAT = 100000000, LONG_IN_PLACE = 160000000;
+// The products of long lists are written past the caches (non-temporal; 580 MB in 16 bits, flat: 425, with plain stores 502) and their
+// gradients read so by k_clip (439 with plain loads), by k_norm_partial from here on: below, the last-level cache keeps some of them for
+// k_clip (flat, plain and past: 240 MB 111 and 117, 500 MB 239 and 246, 580 MB 430 and 425, 1 GB 495 and 492).
+constexpr int64_t PAST_NORM = 540000000;
+// Workgroups of a launch of k_norm_partial, and the most partial sums of a call.
+constexpr int GRID = 2048, LONG_GRID = 1024, PARTS = 2048, LONG_PARTS = 8192;
+// Pieces of a workgroup of k_clip on a long list in place: when the coefficient is 1 they all only come and go (500 MB of fp32 with one
+// piece, four, sixteen: 107, 91, 87 us; with a coefficient below 1 233, 226, 238).
+constexpr int IN_PLACE_PIECES = 4;
 constexpr int SPARSE_MAX = 4;         // row-sparse tensors per launch
 
 struct sparse_grad {
@@ -32,8 +42,9 @@ template <int N, bool FLAT> struct grad_list {
   uint32_t to[FLAT ? N : 1];          // flat: where the tensor begins in its type's buffer, in elements from flat[type]
   char* flat[3];                      // (the buffers, moved on to this list's first tensor of the type)
 };
-typedef grad_list<310, false> in_place_list;
-typedef grad_list<235, true> flat_list;
+constexpr int IN_PLACE_MAX = 310, FLAT_MAX = 235;
+typedef grad_list<IN_PLACE_MAX, false> in_place_list;
+typedef grad_list<FLAT_MAX, true> flat_list;
 static_assert(sizeof(in_place_list) <= 4000 && sizeof(flat_list) <= 4000, "kernel arguments");
 
 struct piece { char* p; int64_t offset; int len, dtype, tensor; };       // offset: bytes from the tensor's beginning
@@ -89,7 +100,7 @@ __device__ __forceinline__ double squares(const u32x4 (&r)[STEPS], const piece& 
   }
   return acc;
 }
-template <bool STREAMS, class T, int STEPS>
+template <bool PAST, class T, int STEPS>
 __device__ __forceinline__ void scale(const u32x4 (&r)[STEPS], const piece& q, char* out, float c) {
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) {
@@ -99,7 +110,7 @@ __device__ __forceinline__ void scale(const u32x4 (&r)[STEPS], const piece& q, c
       unpack16<T>(r[k], f);
 #pragma unroll
       for (int j = 0; j < elems16<T>; ++j) f[j] *= c;
-      if constexpr (STREAMS) store16_past(out + b, pack16<T>(f));
+      if constexpr (PAST) store16_past(out + b, pack16<T>(f));
       else store16(out + b, pack16<T>(f));
     } else {
       for (int e = b; e < q.len; e += (int)sizeof(T))
@@ -107,13 +118,13 @@ __device__ __forceinline__ void scale(const u32x4 (&r)[STEPS], const piece& q, c
     }
   }
 }
-template <bool STREAMS, int STEPS>
+template <bool PAST, int STEPS>
 __device__ __forceinline__ void request(u32x4 (&r)[STEPS], const piece& q) {
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) {
     const int b = ((int)threadIdx.x + 256 * k) * 16;
     if (b + 16 <= q.len) {
-      if constexpr (STREAMS) r[k] = load16_past(q.p + q.offset + b);
+      if constexpr (PAST) r[k] = load16_past(q.p + q.offset + b);
       else r[k] = load16(q.p + q.offset + b);
     }
   }
@@ -129,7 +140,7 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
 }
 
 // The pieces are taken from the last to the first: what was read last is still in the 256 MB last-level cache when k_clip begins.
-template <int BYTES>
+template <int BYTES, bool PAST>
 __global__ __launch_bounds__(256) void k_norm_partial(in_place_list list, double* __restrict__ part) {
   constexpr int STEPS = BYTES / 4096;
   __shared__ double lds[4];
@@ -139,7 +150,7 @@ __global__ __launch_bounds__(256) void k_norm_partial(in_place_list list, double
   for (int i = pieces - 1 - (int)blockIdx.x; i >= 0; i -= (int)gridDim.x) {
     const piece q = where.find(list, i, BYTES);
     u32x4 r[STEPS];
-    request<false>(r, q);
+    request<PAST>(r, q);
     if (q.dtype == ORCA_F32) acc += squares<float>(r, q);
     else if (q.dtype == ORCA_BF16) acc += squares<__bf16>(r, q);
     else acc += squares<_Float16>(r, q);
@@ -150,14 +161,17 @@ __global__ __launch_bounds__(256) void k_norm_partial(in_place_list list, double
 
 // the coefficient from the partial sums: every workgroup adds them in the same order
 __device__ __forceinline__ float coefficient(const double* __restrict__ part, int parts, double max_norm, double* lds, double* norm) {
-  double v[PARTS / 256], acc = 0.0;
+  double acc = 0.0;
+  for (int i0 = 0; i0 < parts; i0 += PARTS) {
+    double v[PARTS / 256];
 #pragma unroll
-  for (int k = 0; k < PARTS / 256; ++k) {
-    const int i = threadIdx.x + 256 * k;
-    v[k] = i < parts ? part[i] : 0.0;
+    for (int k = 0; k < PARTS / 256; ++k) {
+      const int i = i0 + (int)threadIdx.x + 256 * k;
+      v[k] = i < parts ? part[i] : 0.0;
+    }
+#pragma unroll
+    for (int k = 0; k < PARTS / 256; ++k) acc += v[k];
   }
-#pragma unroll
-  for (int k = 0; k < PARTS / 256; ++k) acc += v[k];
   *norm = sqrt(block_sum(acc, lds));
   const double c = max_norm / (*norm + 1e-6);
   return c > 1.0 ? 1.0f : (float)c;       // (a NaN stays one)
@@ -174,8 +188,10 @@ __global__ __launch_bounds__(256) void k_norm_finish(const double* __restrict__ 
   }
 }
 
-template <int BYTES, bool STREAMS, class L, bool FLAT>
-__global__ __launch_bounds__(256) void k_clip(L list, const double* __restrict__ part, int parts, double max_norm, float* __restrict__ norm) {
+// coef (long lists): what k_norm_finish left; else the coefficient is made here
+template <int BYTES, bool PAST, class L, bool FLAT>
+__global__ __launch_bounds__(256) void k_clip(L list, const float* __restrict__ coef, const double* __restrict__ part, int parts, double max_norm,
+                                              float* __restrict__ norm) {
   constexpr int STEPS = BYTES / 4096;
   __shared__ double lds[4];
   const locator<L> where(list);
@@ -183,21 +199,28 @@ __global__ __launch_bounds__(256) void k_clip(L list, const double* __restrict__
   int i = blockIdx.x;
   piece q = where.find(list, i, BYTES);                   // (there are at least as many pieces as workgroups)
   u32x4 r[STEPS];
-  request<STREAMS>(r, q);
-  double n;
-  const float c = coefficient(part, parts, max_norm, lds, &n);
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  float c;
+  if constexpr (BYTES == LONG_PIECE) {
+    c = *coef;
+    if (!FLAT && c == 1.0f) return;
+  }
+  request<PAST>(r, q);
+  if constexpr (BYTES != LONG_PIECE) {
+    double n;
+    c = coefficient(part, parts, max_norm, lds, &n);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  }
   if (!FLAT && c == 1.0f) return;
   for (;;) {
     char* out = q.p + q.offset;
     if constexpr (FLAT) out = list.flat[q.dtype] + (int64_t)list.to[q.tensor] * (q.dtype == ORCA_F32 ? 4 : 2) + q.offset;
-    if (q.dtype == ORCA_F32) scale<STREAMS, float>(r, q, out, c);
-    else if (q.dtype == ORCA_BF16) scale<STREAMS, __bf16>(r, q, out, c);
-    else scale<STREAMS, _Float16>(r, q, out, c);
+    if (q.dtype == ORCA_F32) scale<PAST, float>(r, q, out, c);
+    else if (q.dtype == ORCA_BF16) scale<PAST, __bf16>(r, q, out, c);
+    else scale<PAST, _Float16>(r, q, out, c);
     i += (int)gridDim.x;
     if (i >= pieces) break;
     q = where.find(list, i, BYTES);
-    request<STREAMS>(r, q);
+    request<PAST>(r, q);
   }
 }
 
@@ -213,7 +236,7 @@ struct host_list {
 };
 int64_t bytes_of(const host_list& h, int i) { return h.sizes[i] * (h.dtypes[i] == ORCA_F32 ? 4 : 2); }
 
-int check_list(const char* who, host_list* h, double max_norm, const float* norm, const void* workspace) {
+int check_list(const char* who, host_list* h, int64_t long_from, double max_norm, const float* norm, const void* workspace) {
   ORCA_REQUIRE(h->n >= 0 && h->n <= 65536 && norm && workspace && (h->n == 0 || (h->grads && h->sizes && h->dtypes)) && (!h->rows || h->widths),
                "%s: null argument, or not 0 to 65536 tensors", who);
   ORCA_REQUIRE(((uintptr_t)workspace & 7) == 0, "%s: the workspace is not 8-byte aligned", who);
@@ -227,7 +250,7 @@ int check_list(const char* who, host_list* h, double max_norm, const float* norm
     total += bytes_of(*h, i);
   }
   // small pieces up to four workgroups per CU of them
-  h->piece = total <= 1024LL * SMALL_PIECE ? SMALL_PIECE : PIECE;
+  h->piece = total <= 1024LL * SMALL_PIECE ? SMALL_PIECE : total <= long_from ? PIECE : LONG_PIECE;
   h->pieces = 0;
   for (int i = 0; i < h->n; ++i) h->pieces += ceil_div64(bytes_of(*h, i), h->piece);
   ORCA_REQUIRE(h->pieces < (1LL << 31), "%s: too many elements for one call", who);
@@ -264,18 +287,38 @@ template <class L, bool FLAT> void take(const host_list& h, int* i, int64_t* to,
   }
 }
 
-// k_norm_partial over the list: *parts sums, at most PARTS (each launch gets its share of them)
-int partial_sums(const host_list& h, double* part, int* parts, hipStream_t stream) {
+int launches_of(const host_list& h) {             // how many lists take() makes of it, without flat buffers
+  int launches = 0, n = 0, sparse = 0;
+  for (int i = 0; i < h.n; ++i) {
+    if (h.sizes[i] == 0) continue;
+    const int s = h.rows && h.rows[i];
+    if (launches == 0 || n == IN_PLACE_MAX || sparse + s > SPARSE_MAX) {
+      ++launches;
+      n = sparse = 0;
+    }
+    ++n;
+    sparse += s;
+  }
+  return launches;
+}
+
+// k_norm_partial over the list: *parts sums
+int partial_sums(const char* who, const host_list& h, double* part, int* parts, hipStream_t stream) {
   *parts = 0;
-  const int64_t launches = ceil_div64(h.n, SPARSE_MAX), room = PARTS - std::min<int64_t>(launches, PARTS / 2);
+  const bool is_long = h.piece == LONG_PIECE;
+  const int64_t most = is_long ? LONG_PARTS : PARTS, launches = launches_of(h);
+  ORCA_REQUIRE(launches <= most / 2, "%s: too many row-sparse gradients for one call", who);
   for (int i = 0; i < h.n;) {
     in_place_list list;
     take<in_place_list, false>(h, &i, nullptr, &list);
     if (list.n == 0) continue;
-    const int64_t mine = list.first[list.n], grid = std::min({mine, mine * room / h.pieces + 1, (int64_t)(PARTS - *parts)});
-    ORCA_REQUIRE(grid > 0, "orca_grad_norm: too many row-sparse gradients for one call");
-    if (h.piece == PIECE) k_norm_partial<PIECE><<<(unsigned)grid, 256, 0, stream>>>(list, part + *parts);
-    else k_norm_partial<SMALL_PIECE><<<(unsigned)grid, 256, 0, stream>>>(list, part + *parts);
+    // (shares of what is left when every launch has one)
+    const int64_t mine = list.first[list.n], wanted = is_long ? LONG_GRID : GRID;
+    const unsigned grid = (unsigned)std::min({mine, wanted, launches * wanted <= most ? wanted : mine * (most - launches) / h.pieces + 1});
+    if (is_long && h.pieces * LONG_PIECE >= PAST_NORM) k_norm_partial<LONG_PIECE, true><<<grid, 256, 0, stream>>>(list, part + *parts);
+    else if (is_long) k_norm_partial<LONG_PIECE, false><<<grid, 256, 0, stream>>>(list, part + *parts);
+    else if (h.piece == PIECE) k_norm_partial<PIECE, false><<<grid, 256, 0, stream>>>(list, part + *parts);
+    else k_norm_partial<SMALL_PIECE, false><<<grid, 256, 0, stream>>>(list, part + *parts);
     ORCA_LAUNCH_CHECK();
     *parts += (int)grid;
   }
@@ -283,7 +326,7 @@ int partial_sums(const host_list& h, double* part, int* parts, hipStream_t strea
 }
 
 template <class L, bool FLAT>
-int clip(const host_list& h, void* const* flat, const double* part, int parts, double max_norm, float* norm, hipStream_t stream) {
+int clip(const host_list& h, void* const* flat, const float* coef, const double* part, int parts, double max_norm, float* norm, hipStream_t stream) {
   int64_t to[3] = {0, 0, 0};
   for (int i = 0; i < h.n;) {
     L list;
@@ -291,10 +334,10 @@ int clip(const host_list& h, void* const* flat, const double* part, int parts, d
       for (int k = 0; k < 3; ++k) list.flat[k] = (char*)flat[k] + to[k] * (k == ORCA_F32 ? 4 : 2);
     take<L, FLAT>(h, &i, to, &list);
     if (list.n == 0) continue;
-    const unsigned grid = (unsigned)std::min(list.first[list.n], 2048);
-    if (h.piece == SMALL_PIECE) k_clip<SMALL_PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, part, parts, max_norm, norm);
-    else if (FLAT && h.pieces * h.piece > STREAM_BYTES) k_clip<PIECE, FLAT, L, FLAT><<<grid, 256, 0, stream>>>(list, part, parts, max_norm, norm);
-    else k_clip<PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, part, parts, max_norm, norm);
+    const unsigned pieces = (unsigned)list.first[list.n], grid = std::min<unsigned>(pieces, GRID);
+    if (h.piece == LONG_PIECE) k_clip<LONG_PIECE, true, L, FLAT><<<FLAT ? pieces : (pieces - 1) / IN_PLACE_PIECES + 1, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
+    else if (h.piece == PIECE) k_clip<PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
+    else k_clip<SMALL_PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
     ORCA_LAUNCH_CHECK();
     norm = nullptr;             // (the first launch writes it)
   }
@@ -302,15 +345,15 @@ int clip(const host_list& h, void* const* flat, const double* part, int parts, d
 }
 }  // namespace
 
-ORCA_API int64_t orca_grad_norm_workspace_bytes(void) { return PARTS * 8; }
+ORCA_API int64_t orca_grad_norm_workspace_bytes(void) { return LONG_PARTS * 8 + 8; }
 
 ORCA_API int orca_grad_norm(int n, void* const* grads, const int64_t* sizes, const uint8_t* dtypes, const int32_t* const* rows, const int32_t* widths,
                             double max_norm, float* norm, float* coef, void* workspace, void* stream_) {
   hipStream_t stream = (hipStream_t)stream_;
   host_list h{n, grads, sizes, dtypes, rows, widths, 0, 0};
   int parts = 0;
-  if (int rc = check_list("orca_grad_norm", &h, max_norm, norm, workspace)) return rc;
-  if (int rc = partial_sums(h, (double*)workspace, &parts, stream)) return rc;
+  if (int rc = check_list("orca_grad_norm", &h, LONG_IN_PLACE, max_norm, norm, workspace)) return rc;
+  if (int rc = partial_sums("orca_grad_norm", h, (double*)workspace, &parts, stream)) return rc;
   k_norm_finish<<<1, 256, 0, stream>>>((const double*)workspace, parts, max_norm, norm, coef);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
@@ -321,15 +364,15 @@ ORCA_API int orca_clip_grads(int n, void* const* grads, const int64_t* sizes, co
   hipStream_t stream = (hipStream_t)stream_;
   host_list h{n, grads, sizes, dtypes, rows, widths, 0, 0};
   int parts = 0;
-  if (int rc = check_list("orca_clip_grads", &h, max_norm, norm, workspace)) return rc;
+  if (int rc = check_list("orca_clip_grads", &h, flat ? LONG_FLAT : LONG_IN_PLACE, max_norm, norm, workspace)) return rc;
   for (int i = 0; flat && i < n; ++i) ORCA_REQUIRE(sizes[i] == 0 || flat[dtypes[i]], "orca_clip_grads: no flat buffer for type %d", dtypes[i]);
-  if (int rc = partial_sums(h, (double*)workspace, &parts, stream)) return rc;
+  if (int rc = partial_sums("orca_clip_grads", h, (double*)workspace, &parts, stream)) return rc;
   const double* part = (const double*)workspace;
-  if (h.pieces == 0) {
-    k_norm_finish<<<1, 256, 0, stream>>>(part, 0, max_norm, norm, nullptr);
+  float* coef = (float*)((double*)workspace + LONG_PARTS);
+  if (h.pieces == 0 || h.piece == LONG_PIECE) {
+    k_norm_finish<<<1, 256, 0, stream>>>(part, parts, max_norm, norm, coef);
     ORCA_LAUNCH_CHECK();
-    return ORCA_OK;
   }
-  return flat ? clip<flat_list, true>(h, flat, part, parts, max_norm, norm, stream)
-              : clip<in_place_list, false>(h, flat, part, parts, max_norm, norm, stream);
+  return flat ? clip<flat_list, true>(h, flat, coef, part, parts, max_norm, norm, stream)
+              : clip<in_place_list, false>(h, flat, coef, part, parts, max_norm, norm, stream);
 }

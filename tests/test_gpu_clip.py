@@ -268,3 +268,35 @@ def test_on_another_stream(ops):
     n1 = ops.clip_grad_norm(got, 0.5)
   s.synchronize()
   assert torch.equal(n0, n1) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("flat", [True, False])
+@pytest.mark.parametrize("parts", [1, 700])
+def test_long_lists(ops, flat, parts):
+  """170 MB (three launches, a piece or four per workgroup) as one tensor and as hundreds, odd sizes, with a row-sparse one in front"""
+  sizes = [85000001 // parts + (i % 3) for i in range(parts)]
+  base = torch.randn(sum(sizes), device=DEV, generator=torch.Generator(DEV).manual_seed(parts)).bfloat16()
+  grads, at = [], 0
+  for k in sizes:
+    grads.append(base[at:at + k])
+    at += k
+  rows = ops.RowGrad(torch.arange(50, device=DEV), torch.full((50, 7), 3.0, device=DEV), torch.full((1,), 20, dtype=torch.int32, device=DEV), 50)
+  want = float((base.double().square().sum() + 140 * 9.0).sqrt())
+  before, out = base.clone(), [torch.full((350,), 8.0, device=DEV), torch.empty_like(base)]
+  max_norm = want / 3
+  norm = ops.clip_grad_norm([rows] + grads, max_norm, flat=out if flat else None)
+  # the norm: fp64 sums, one rounding to fp32.  The products: a coefficient rounded to fp32, one product, one rounding to bf16
+  assert abs(float(norm) - want) <= want * 2 * U
+  exp = before.double() * (max_norm / (want + 1e-6))
+  got = (out[1] if flat else base).double()
+  assert bool(((got - exp).abs() <= exp.abs() * (2.0 ** -8 + 4 * U)).all())
+  r = out[0] if flat else rows.rows.reshape(-1)
+  assert bool(((r[:140] - 1.0).abs() <= 4 * U + 1e-6 / want * 2).all()) and bool((r[140:] == (8.0 if flat else 3.0)).all())
+  if flat:
+    assert torch.equal(base, before)
+  else:
+    again = base.clone()
+    ops.clip_grad_norm(grads, 1e9)
+    assert torch.equal(base, again)
+  n1, c = ops.grad_norm([before] if parts == 1 else [g.clone() for g in grads], max_norm)
+  assert bool(torch.isfinite(n1)) and 0 < float(c) < 1
