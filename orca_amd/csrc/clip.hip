@@ -4,7 +4,8 @@
 // adds those sums up in the same order (while its first piece is on its way) before it scales its share.  Long ones, where that time
 // shows: k_norm_finish adds them up in between, and a workgroup of k_clip takes a piece or four and ends.  Squares and sums are fp64:
 // neither overflows nor vanishes for any fp32 input, and the conversions hide behind the loads (4.5 elements per clock and CU at the
-// HBM rate for 16-bit gradients).
+// HBM rate for 16-bit gradients).  Bound by the HBM: 400 million elements in 300 tensors, 580 MB, 425 us = 138 (4.2 TB/s) + 5 + 282 (4.1
+// TB/s); short lists by the two launches: 35 tensors of 2.9 MB 3.5 + 4.6 us.
 //   A list travels in the kernel's arguments, under 4 KB: 12 bytes per tensor (16 with flat buffers), so that a few hundred tensors
 // are one launch.  With a search by scalar loads through 41 bytes per tensor, k_norm_partial took 6.4 us for 32 tensors of 2.9 MB.
 #include <algorithm>
@@ -334,8 +335,8 @@ int clip(const host_list& h, void* const* flat, const float* coef, const double*
       for (int k = 0; k < 3; ++k) list.flat[k] = (char*)flat[k] + to[k] * (k == ORCA_F32 ? 4 : 2);
     take<L, FLAT>(h, &i, to, &list);
     if (list.n == 0) continue;
-    const unsigned pieces = (unsigned)list.first[list.n], grid = std::min<unsigned>(pieces, GRID);
-    if (h.piece == LONG_PIECE) k_clip<LONG_PIECE, true, L, FLAT><<<FLAT ? pieces : (pieces - 1) / IN_PLACE_PIECES + 1, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
+    const unsigned pieces = (unsigned)list.first[list.n], grid = std::min<unsigned>(pieces, GRID), many = FLAT ? pieces : (pieces - 1) / IN_PLACE_PIECES + 1;
+    if (h.piece == LONG_PIECE) k_clip<LONG_PIECE, true, L, FLAT><<<many, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
     else if (h.piece == PIECE) k_clip<PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
     else k_clip<SMALL_PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
     ORCA_LAUNCH_CHECK();

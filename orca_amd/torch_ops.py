@@ -227,7 +227,8 @@ _lib.register_autograd("orca::history_pull_pushed", _hpp_backward, setup_context
 # ---- a learned table: lookup with its gradient ------------------------------------------------------------------
 @_lib.custom_op("orca::embedding", mutates_args=())
 def embedding(table: Tensor, ids: Tensor, scale: float, padding_idx: int) -> Tensor:
-  """scale * table[ids]; the row of padding_idx (negative: none) reads like any other and gets no gradient"""
+  """scale * table[ids]; the row of padding_idx (negative: none) reads like any other and gets no gradient.  (A captured
+  backward pass: as anywhere in torch, no eager graph of the same leaves may be alive.)"""
   return ops.embedding(table, ids, scale)
 
 
