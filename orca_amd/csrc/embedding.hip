@@ -615,7 +615,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_segment_join(seg_args a) {
 }
 
 // ---- short lists -----------------------------------------------------------------------------------------------------
-// Up to SMALL_N ids (and SMALL_VALUES values) there is no order of the whole list to build: every workgroup reads all the ids (26 KB
+// Up to SMALL_N ids and SMALL_VALUES values there is no order of the whole list to build: every workgroup reads all the ids (26 KB
 // for 6600 of them, out of L2), keeps its share in the order of their positions and sorts those few in LDS.
 //   dense, one launch (k_small): a hash of the id gives it to a workgroup, which adds its ids' rows.  It also has a share of the
 //          table's rows; it marks those with an occurrence and zeroes the others, so that every row is written once.
@@ -628,7 +628,10 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_segment_join(seg_args a) {
 // took 24 us.
 constexpr int SMALL_THREADS = 1024, SMALL_ITEMS = 8, SMALL_N = SMALL_THREADS * SMALL_ITEMS;
 constexpr int TINY_THREADS = 256, TINY_N = TINY_THREADS * SMALL_ITEMS;         // workgroups of four waves: cheaper barriers
-constexpr int64_t SMALL_VALUES = 1 << 20;      // beyond, a hub id's rows are too many for the one workgroup that adds them
+// Most values, us here and on the general path (row-sparse, dense; 1/rank ids): 2^21 (1000 ids of 2048 fp32) 19 and 29, 17 and 34; 2^23
+// (2000 of 4096) 27 and 39, 27 and 48; 2^24 (8000 of 2048) 45 and 50, 35 and 50.  The small workgroups are the faster ones for the rows of
+// 2^20 (250 of 4096: 12.6 and 14.3), not for 2^21.
+constexpr int64_t SMALL_VALUES = 1 << 24, TINY_VALUES = 1 << 20;
 constexpr int SMALL_MAP = 65536;               // table rows of a workgroup's share, at most (bits in LDS)
 constexpr int SMALL_RUN = 32;                  // a longer run of equal ids is added by the whole workgroup ...
 constexpr int SMALL_TEAMS = 32;                // ... in at most this many consecutive parts
@@ -1137,16 +1140,19 @@ int launch_sums(seg_args a, bool accumulate, hipStream_t stream) {
   return ORCA_OK;
 }
 
+bool is_tiny(int64_t n, int64_t width) { return n <= TINY_N && n * width <= TINY_VALUES; }        // for the small workgroups
 bool is_small(int64_t n, int64_t width) { return n <= SMALL_N && n * width <= SMALL_VALUES; }
 // Whether k_small's workgroups mark the rows and zero the others: as many rows as they can mark, and no more bytes than pay a launch of
 // its own, whose stores run at the full rate.  Marked and filled ahead, us, workgroups of 256 threads (20 ids in rows of 49 fp32): 16 MB 9.0
 // and 8.5, 24 MB 10.9 and 9.3, 64 MB 19.6 and 14.3 (rows of 256 bf16: 8.2 and 8.7, 9.6 and 9.8, 15.9 and 14.3); of 1024 threads (2500 ids in
 // rows of 8 fp32): 24 MB 15.0 and 16.7, 64 MB 20.4 and 22.4, 128 MB 27.6 and 30.1, 160 MB 33.4 and 33.8.
-bool maps(int64_t n, int64_t num_rows, int64_t bytes) { return num_rows <= 256LL * SMALL_MAP && bytes <= (n <= TINY_N ? 20 : 160) * MB; }
+bool maps(bool tiny, int64_t num_rows, int64_t bytes) { return num_rows <= 256LL * SMALL_MAP && bytes <= (tiny ? 20 : 160) * MB; }
 template <class T> void columns(small_args* a) {
   constexpr int VEC = elems16<T>;
   a->chunks = a->width < VEC ? a->width : (a->width + VEC - 1) / VEC;
-  a->log_l = log_lanes(a->chunks, 6);
+  // half a wave per row and column block, so that a hub's rows meet more teams (8000 rows of one id, 256 and 2048 fp32: 83 and 86 us, 136
+  // and 140 with whole waves; of uniform ids 16 and 38, 16 and 34), while that leaves 16 shares of the ids (2000 ids of 8000 fp32 40, halves 49)
+  a->log_l = log_lanes(a->chunks, a->chunks <= 512 ? 5 : 6);
   a->col_blocks = (int)ceil_div64(a->chunks, 1 << a->log_l);
 }
 int key_bits(int64_t num_rows) {
@@ -1205,13 +1211,13 @@ int small_rows(small_args a, char* ws, int64_t* ids, int32_t* count, hipStream_t
   int64_t bytes;
   const range_work w = range_layout(ws, a.n, &bytes);
   const int ranges = (int)std::min<int64_t>(MAX_RANGES, ceil_div64(a.n, 4));
-  if (int rc = a.n <= TINY_N ? launch_range_sort<TINY_THREADS>(a, w, ranges, stream) : launch_range_sort<SMALL_THREADS>(a, w, ranges, stream)) return rc;
+  if (int rc = is_tiny(a.n, a.width) ? launch_range_sort<TINY_THREADS>(a, w, ranges, stream) : launch_range_sort<SMALL_THREADS>(a, w, ranges, stream)) return rc;
   // a run per team, no more than are looked up at once, and at most a workgroup per CU (two small ones; one for each column block)
-  const int threads = a.n <= TINY_N ? TINY_THREADS : SMALL_THREADS;
+  const int threads = is_tiny(a.n, a.width) ? TINY_THREADS : SMALL_THREADS;
   const int64_t runs = std::min(RANGE_RUNS, threads >> a.log_l);
-  const int64_t shares = std::max<int64_t>(1, std::min(ceil_div64(a.n, runs), ceil_div64(a.n <= TINY_N ? 512 : 256, a.col_blocks)));
+  const int64_t shares = std::max<int64_t>(1, std::min(ceil_div64(a.n, runs), ceil_div64(is_tiny(a.n, a.width) ? 512 : 256, a.col_blocks)));
   const unsigned grid = (unsigned)(shares * a.col_blocks);
-  auto* kernel = a.n <= TINY_N ? (a.width >= VEC ? k_range_sums<TINY_THREADS, TI, TO, VEC> : k_range_sums<TINY_THREADS, TI, TO, 1>)
+  auto* kernel = is_tiny(a.n, a.width) ? (a.width >= VEC ? k_range_sums<TINY_THREADS, TI, TO, VEC> : k_range_sums<TINY_THREADS, TI, TO, 1>)
                                : (a.width >= VEC ? k_range_sums<SMALL_THREADS, TI, TO, VEC> : k_range_sums<SMALL_THREADS, TI, TO, 1>);
   kernel<<<grid, (unsigned)threads, 0, stream>>>(a, w, ranges, ids, count);
   ORCA_LAUNCH_CHECK();
@@ -1329,14 +1335,14 @@ ORCA_API int orca_embedding_backward(const void* grad_out, int grad_dtype, int64
     fill.past = past_zeros(num_rows * width * e);
   }
   if (n == 0) return launch_fill(fill, pieces, stream);
-  const bool marks = !accumulate && maps(n, num_rows, num_rows * width * (table_dtype == ORCA_F32 ? 4 : 2));
+  const bool marks = !accumulate && maps(is_tiny(n, width), num_rows, num_rows * width * (table_dtype == ORCA_F32 ? 4 : 2));
   if (is_small(n, width)) {
     if (!accumulate && !marks) {
       if (int rc = launch_fill(fill, pieces, stream)) return rc;
     }
     const small_args a{idx64, idx32, num_rows, padding_idx, grad_out, ld_grad, ld_table, grad_table, (int)n, (int)width, 0, 0, 0, marks, scale};
     return by_types(grad_dtype, table_dtype, [&](auto gi, auto go) {
-      return n <= TINY_N ? small_dense<TINY_THREADS, decltype(gi), decltype(go)>(a, accumulate != 0, stream)
+      return is_tiny(n, width) ? small_dense<TINY_THREADS, decltype(gi), decltype(go)>(a, accumulate != 0, stream)
                          : small_dense<SMALL_THREADS, decltype(gi), decltype(go)>(a, accumulate != 0, stream);
     });
   }

@@ -505,3 +505,23 @@ def test_zeros_of_strided_tables(ops):
       check_grad(buf[:, :w], grad, ids, vocab, 1.0, None)
     else:
       assert int((buf[:, :w] != 0).any(1).sum()) == torch.unique(ids).numel()
+
+
+@pytest.mark.parametrize("n,width,t", [(8192, 2048, torch.float32), (2000, 8001, torch.bfloat16), (250, 65536, torch.float32), (2049, 513, torch.float16),
+                                       (2048, 512, torch.float32), (2048, 513, torch.float32), (1500, 4099, torch.bfloat16), (64, 8192, torch.float16)])
+@pytest.mark.parametrize("kind", ["hubs", "same"])
+def test_short_lists_of_wide_rows(ops, n, width, t, kind):
+  """rows over many column blocks, up to the most values that a short list has, and their sums again"""
+  vocab = 300
+  g = torch.Generator(device=DEV).manual_seed(n + width)
+  ids = make_ids(kind, n, vocab, n).clamp_(max=vocab - 1).to(DEV)
+  grad = torch.empty(n, width, device=DEV).normal_(generator=g).to(t)
+  got = ops.embedding_backward(grad, ids, vocab, scale=0.5)
+  G = torch.zeros(vocab, width, device=DEV, dtype=torch.float64).index_add_(0, ids, grad.double()).mul_(0.5)
+  S = torch.zeros(vocab, width, device=DEV, dtype=torch.float64).index_add_(0, ids, grad.double().abs()).mul_(0.5)
+  m = torch.bincount(ids, minlength=vocab)[:, None]
+  assert bool(((got.double() - G).abs() <= 1.01 * ((m + 2) * U * S + half(t) * G.abs()) + tiny(t)).all())
+  rg = ops.embedding_backward_rows(grad, ids, vocab, scale=0.5)
+  k = int(rg.count)
+  assert torch.equal(rg.ids[:k], torch.unique(ids)) and torch.equal(rg.rows[:k], got[rg.ids[:k]])
+  assert torch.equal(ops.embedding_backward(grad, ids, vocab, scale=0.5), got)
