@@ -693,21 +693,22 @@ class FusedAdam:
     norm = coef = None
     if max_norm is not None:
       norm, coef = grad_norm(used, max_norm)
-    by_step = {}
-    for k, g in used.items():
-      self.steps[k] += 1
-      if isinstance(g, RowGrad):
-        check(_lib.load().orca_adam_rows(ptr(g.ids), ptr(g.rows), ptr(g.count), g.ids.numel(), g.num_rows, g.rows.shape[1], ptr(self.params[k]),
-                                         ptr(self.exp_avg[k]), ptr(self.exp_avg_sq[k]), self.lr, self.betas[0], self.betas[1], self.eps,
-                                         self.steps[k], ptr(coef), stream()), "orca_adam_rows")
-      else:
-        by_step.setdefault(self.steps[k], []).append((self.params[k], g, self.exp_avg[k], self.exp_avg_sq[k]))
-    for t, lst in by_step.items():
-      n = len(lst)
-      arr = lambda j: (ctypes.c_void_p * n)(*[x[j].data_ptr() for x in lst])
-      sizes = (ctypes.c_int64 * n)(*[x[0].numel() for x in lst])
-      check(_lib.load().orca_adam_step_scaled(n, arr(0), arr(1), arr(2), arr(3), sizes, self.lr, self.betas[0], self.betas[1],
-                                              self.eps, t, ptr(coef), stream()), "orca_adam_step")
+    with torch.cuda.device(self._state.device):
+      by_step = {}
+      for k, g in used.items():
+        self.steps[k] += 1
+        if isinstance(g, RowGrad):
+          check(_lib.load().orca_adam_rows(ptr(g.ids), ptr(g.rows), ptr(g.count), g.ids.numel(), g.num_rows, g.rows.shape[1], ptr(self.params[k]),
+                                           ptr(self.exp_avg[k]), ptr(self.exp_avg_sq[k]), self.lr, self.betas[0], self.betas[1], self.eps,
+                                           self.steps[k], ptr(coef), stream()), "orca_adam_rows")
+        else:
+          by_step.setdefault(self.steps[k], []).append((self.params[k], g, self.exp_avg[k], self.exp_avg_sq[k]))
+      for t, lst in by_step.items():
+        n = len(lst)
+        arr = lambda j: (ctypes.c_void_p * n)(*[x[j].data_ptr() for x in lst])
+        sizes = (ctypes.c_int64 * n)(*[x[0].numel() for x in lst])
+        check(_lib.load().orca_adam_step_scaled(n, arr(0), arr(1), arr(2), arr(3), sizes, self.lr, self.betas[0], self.betas[1],
+                                                self.eps, t, ptr(coef), stream()), "orca_adam_step")
     return norm
 
 

@@ -525,3 +525,34 @@ def test_short_lists_of_wide_rows(ops, n, width, t, kind):
   k = int(rg.count)
   assert torch.equal(rg.ids[:k], torch.unique(ids)) and torch.equal(rg.rows[:k], got[rg.ids[:k]])
   assert torch.equal(ops.embedding_backward(grad, ids, vocab, scale=0.5), got)
+
+
+def test_autograd_captured(ops):
+  """forward and backward in one graph (no eager graph of the leaf is alive), replayed with other contents beside eager work"""
+  from orca_amd import torch_ops  # noqa: F401
+  vocab, w, n = 900, 24, 1500
+  table = torch.randn(vocab, w, device=DEV).requires_grad_()
+  ids, wgt = torch.zeros(n, dtype=torch.int64, device=DEV), torch.zeros(n, w, device=DEV)
+
+  def step():
+    out = torch.ops.orca.embedding(table, ids, 0.5, 0)
+    return torch.autograd.grad(out, table, wgt)[0]
+
+  s = torch.cuda.Stream()
+  s.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(s):
+    for _ in range(2):
+      step()
+  torch.cuda.current_stream().wait_stream(s)
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    grad = step()
+  for r in range(3):
+    g = torch.Generator().manual_seed(r)
+    ids.copy_(torch.randint(0, vocab, (n,), generator=g))
+    wgt.copy_(torch.randn(n, w, generator=g))
+    graph.replay()
+    torch.cuda.synchronize()
+    check_grad(grad, wgt, ids, vocab, 0.5, 0)
+    assert torch.equal(grad, ops.embedding_backward(wgt, ids, vocab, 0.5, 0)), f"replay {r}"
