@@ -6,6 +6,7 @@
 // occurrences is spread over as many windows as it needs and two runs give the same bits.  (orca_scatter_add_flagged adds with
 // fp32 atomics in whatever order they arrive.)
 #include <algorithm>
+#include <type_traits>
 #include "elem.h"
 
 namespace {
@@ -141,14 +142,18 @@ __global__ __launch_bounds__(256) void k_fill(fill_job f) { fill_pieces<256>(f, 
 
 // ---- sort of the positions by id -------------------------------------------------------------------------------------
 // Stable least-significant-digit radix sort of (key, position) pairs; key = the id, or num_rows for what has no row (the padding
-// id, ids outside the table): those end up last and are dropped.  A tile is SORT_TILE consecutive pairs of one workgroup; within it
-// a wave owns 64 * SORT_ITEMS consecutive pairs and ranks them 64 at a time: the lanes with the same digit find each other with one
+// id, ids outside the table): those end up last and are dropped.  A tile is 512 * ITEMS consecutive pairs of one workgroup; within it
+// a wave owns 64 * ITEMS consecutive pairs and ranks them 64 at a time: the lanes with the same digit find each other with one
 // ballot per digit bit.  Two launches per pass (count, scatter); with many tiles a third one adds the counts up.  Bound by latency: 85,995
-// pairs in digits of 8 bits 4.1 and 7.4 us a pass; with 100 MB of zeros on board 16.4 and 16.0 (6.2 TB/s).
-constexpr int SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS;
+// pairs in digits of 8 bits 4.1 and 7.6 us a pass; with 100 MB of zeros on board 16.4 and 16.0 (6.2 TB/s).
+constexpr int SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64;
 constexpr int MIN_DIGIT = 2, MAX_DIGIT = 11, MAX_BINS = 1 << MAX_DIGIT;
-constexpr int DIRECT_TILES = 64;        // up to this many tiles every workgroup adds the counts up itself
-static_assert(SORT_TILE <= 65536, "16-bit counts within a tile");
+// Up to this many tiles every workgroup adds the tiles' counts up itself; it takes the fewest pairs per thread whose counts stay below the
+// bytes for one and for two.  One, two and four, us, row-sparse: 12,000 pairs in digits of 7 bits 29 31 36, 20,000 of 10 bits 38 39 43, 45,000 of
+// 10 42 40 43, 86,000 of 8 52 53 57, 131,072 of 11 93 67 58, 300,000 of 10 133 93 75.
+constexpr int DIRECT_TILES = 64;
+constexpr int64_t ONE_BYTES = 192000, TWO_BYTES = 256000;
+static_assert(4 * SORT_THREADS <= 65536, "16-bit counts within a tile");
 static_assert(2 * SORT_THREADS * 16 <= SORT_WAVES * MAX_BINS * 2, "the slices' sums fit where the counts lie");
 static_assert(MAX_BINS == 4 * SORT_THREADS, "a thread takes four neighbouring bins");
 struct pair32 { uint32_t pos, key; };
@@ -167,23 +172,24 @@ __device__ __forceinline__ pair32 sort_read(const sort_src& s, int64_t i) {
 }
 
 // counts[tile][bin] of this pass' digit
+template <int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void k_sort_count(sort_src src, int shift, int bins, uint32_t* __restrict__ counts, int tiles, fill_job fill) {
   __shared__ uint32_t h[MAX_BINS];
   if ((int)blockIdx.x >= tiles) {
     fill_pieces<SORT_THREADS>(fill, (int)blockIdx.x - tiles, (int)gridDim.x - tiles);
     return;
   }
-  pair32 p[SORT_ITEMS];
-  const int64_t base = (int64_t)blockIdx.x * SORT_TILE;
+  pair32 p[ITEMS];
+  const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ITEMS);
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u) {
+  for (int u = 0; u < ITEMS; ++u) {
     const int64_t i = base + threadIdx.x + SORT_THREADS * u;
     p[u] = i < src.n ? sort_read(src, i) : pair32{0u, 0u};
   }
   for (int b = threadIdx.x; b < bins; b += SORT_THREADS) h[b] = 0;
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u)
+  for (int u = 0; u < ITEMS; ++u)
     if (base + threadIdx.x + SORT_THREADS * u < src.n) atomicAdd(&h[(p[u].key >> shift) & (bins - 1)], 1u);
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += SORT_THREADS) counts[(int64_t)blockIdx.x * bins + b] = h[b];
@@ -235,6 +241,7 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, int digit_bits, bool 
 }
 
 // totals == null: counts holds every tile's counts, which this workgroup adds up itself
+template <int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int shift, int digit_bits, const uint32_t* __restrict__ counts,
                                                                const uint32_t* __restrict__ totals, pair32* __restrict__ out, int tiles, fill_job fill) {
   __shared__ uint32_t place[MAX_BINS];                   // where the tile's first pair of a digit goes
@@ -245,10 +252,10 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
     return;
   }
   const int bins = 1 << digit_bits, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int64_t base = (int64_t)blockIdx.x * SORT_TILE + wave * (64 * SORT_ITEMS);
-  pair32 p[SORT_ITEMS];
+  const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ITEMS) + wave * (64 * ITEMS);
+  pair32 p[ITEMS];
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u) {
+  for (int u = 0; u < ITEMS; ++u) {
     const int64_t i = base + 64 * u + lane;
     p[u] = i < src.n ? sort_read(src, i) : pair32{0u, 0u};
   }
@@ -287,9 +294,9 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
   if (slice != 0) total = u32x4{0, 0, 0, 0};
   for (int k = t; k < SORT_WAVES * MAX_BINS / 8; k += SORT_THREADS) reinterpret_cast<u32x4*>(&part[0][0])[k] = u32x4{0, 0, 0, 0};
   __syncthreads();
-  uint32_t rank[SORT_ITEMS];
+  uint32_t rank[ITEMS];
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u) {
+  for (int u = 0; u < ITEMS; ++u) {
     const bool in = base + 64 * u + lane < src.n;
     const uint32_t d = (p[u].key >> shift) & (uint32_t)(bins - 1);
     const uint64_t peers = same_digit(d, digit_bits, in);
@@ -328,7 +335,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
   }
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u) {
+  for (int u = 0; u < ITEMS; ++u) {
     if (base + 64 * u + lane < src.n) {
       const uint32_t d = (p[u].key >> shift) & (uint32_t)(bins - 1);
       out[place[d] + part[wave][d] + rank[u]] = p[u];
@@ -338,19 +345,20 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_scatter(sort_src src, int
 
 // ---- the rows' numbers (row-sparse form) -----------------------------------------------------------------------------
 // rank[i] = the number of the distinct id that sorted pair i belongs to; ids[rank] = that id; *count = how many there are.  Two launches,
-// as the sort's: heads per tile, then every tile adds up those before it (85,995 pairs: 3.8 and 4.8 us, latency).
+// as the sort's: heads per tile, then every tile adds up those before it (85,995 pairs: 2.1 and 3.4 us, latency).
 __device__ __forceinline__ bool is_head(const pair32* s, int64_t i, uint32_t none) {
   const uint32_t k = s[i].key;
   return k != none && (i == 0 || s[i - 1].key != k);
 }
+template <int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void k_rank_count(const pair32* __restrict__ s, int64_t n, uint32_t none, uint32_t* __restrict__ tile_heads) {
   __shared__ int total;
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * SORT_TILE;
+  const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ITEMS);
   int c = 0;
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u) {
+  for (int u = 0; u < ITEMS; ++u) {
     const int64_t i = base + threadIdx.x + SORT_THREADS * u;
     const uint64_t m = __ballot(i < n && is_head(s, i, none));
     c += __popcll(m);
@@ -359,6 +367,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_rank_count(const pair32* __res
   __syncthreads();
   if (threadIdx.x == 0) tile_heads[blockIdx.x] = (uint32_t)total;
 }
+template <int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void k_rank(const pair32* __restrict__ s, int64_t n, uint32_t none, const uint32_t* __restrict__ tile_heads,
                                                        uint32_t* __restrict__ rank, int64_t* __restrict__ ids, int32_t* __restrict__ count) {
   __shared__ uint32_t before, wave_heads[SORT_WAVES];
@@ -370,11 +379,11 @@ __global__ __launch_bounds__(SORT_THREADS) void k_rank(const pair32* __restrict_
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
   if (lane == 0) atomicAdd(&before, sum);
-  const int64_t base = (int64_t)blockIdx.x * SORT_TILE + wave * (64 * SORT_ITEMS);
-  uint64_t heads[SORT_ITEMS];
+  const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ITEMS) + wave * (64 * ITEMS);
+  uint64_t heads[ITEMS];
   uint32_t mine = 0;
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u) {
+  for (int u = 0; u < ITEMS; ++u) {
     const int64_t i = base + 64 * u + lane;
     heads[u] = __ballot(i < n && is_head(s, i, none));
     mine += (uint32_t)__popcll(heads[u]);
@@ -384,7 +393,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_rank(const pair32* __restrict_
   uint32_t run = before;
   for (int w = 0; w < wave; ++w) run += wave_heads[w];
 #pragma unroll
-  for (int u = 0; u < SORT_ITEMS; ++u) {
+  for (int u = 0; u < ITEMS; ++u) {
     const int64_t i = base + 64 * u + lane;
     const uint32_t upto = run + (uint32_t)__popcll(heads[u] & (~0ULL >> (63 - lane)));      // heads at or before this lane
     if (i < n && s[i].key != none) {
@@ -1068,14 +1077,17 @@ __global__ __launch_bounds__(THREADS) void k_range_sums(small_args a, range_work
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-struct sort_plan { int passes, digit; int64_t tiles; };
+struct sort_plan { int passes, digit, items; int64_t tiles; };
 sort_plan plan_sort(int64_t n, int64_t num_rows) {
   int bits = 1;
   while (bits < 32 && (num_rows >> bits) != 0) ++bits;        // keys 0 .. num_rows
   sort_plan s;
   s.passes = (bits + MAX_DIGIT - 1) / MAX_DIGIT;
   s.digit = std::max(MIN_DIGIT, (bits + s.passes - 1) / s.passes);
-  s.tiles = ceil_div64(n, SORT_TILE);
+  for (s.items = 1;; s.items *= 2) {
+    s.tiles = ceil_div64(n, SORT_THREADS * s.items);
+    if (s.items == 4 || (s.tiles * 4 << s.digit) <= (s.items == 1 ? ONE_BYTES : TWO_BYTES)) break;
+  }
   return s;
 }
 int log_lanes(int64_t chunks, int most) {       // the smallest team that holds a row's chunks, at most 2^most lanes
@@ -1268,24 +1280,35 @@ int launch_fill(fill_job f, int64_t pieces, hipStream_t stream) {
   return ORCA_OK;
 }
 
+template <class F> void by_items(int items, F f) {
+  if (items == 1) f(std::integral_constant<int, 1>{});
+  else if (items == 2) f(std::integral_constant<int, 2>{});
+  else f(std::integral_constant<int, 4>{});
+}
+
 // sorts (id, position), zeroes the fill's pieces on the way; *sorted = where the result lies
 int sort_positions(const int64_t* idx64, const int32_t* idx32, int64_t n, int64_t num_rows, int64_t padding, char* ws, const work_layout& l,
                    fill_job fill, int64_t pieces, const pair32** sorted, hipStream_t stream) {
   const sort_plan s = plan_sort(n, num_rows);
   sort_src src{idx64, idx32, nullptr, n, num_rows, padding};
   uint32_t* counts = (uint32_t*)(ws + l.counts);
-  uint32_t* totals = s.tiles > DIRECT_TILES ? (uint32_t*)(ws + l.totals) : nullptr;
+  uint32_t* totals = s.items == 4 && s.tiles > DIRECT_TILES ? (uint32_t*)(ws + l.totals) : nullptr;
   pair32* buf[2] = {(pair32*)(ws + l.a), (pair32*)(ws + l.b)};
   for (int p = 0; p < s.passes; ++p) {
     unsigned extra = fill_share(&fill, pieces, SORT_THREADS, 2 * p, 2 * s.passes);
-    k_sort_count<<<(unsigned)s.tiles + extra, SORT_THREADS, 0, stream>>>(src, p * s.digit, 1 << s.digit, counts, (int)s.tiles, fill);
+    by_items(s.items, [&](auto items) {
+      k_sort_count<items><<<(unsigned)s.tiles + extra, SORT_THREADS, 0, stream>>>(src, p * s.digit, 1 << s.digit, counts, (int)s.tiles, fill);
+    });
     ORCA_LAUNCH_CHECK();
     if (totals) {
       k_sort_columns<<<((1 << s.digit) + 63) / 64, 64, 0, stream>>>(counts, s.tiles, 1 << s.digit, totals);
       ORCA_LAUNCH_CHECK();
     }
     extra = fill_share(&fill, pieces, SORT_THREADS, 2 * p + 1, 2 * s.passes);
-    k_sort_scatter<<<(unsigned)s.tiles + extra, SORT_THREADS, 0, stream>>>(src, p * s.digit, s.digit, counts, totals, buf[p & 1], (int)s.tiles, fill);
+    by_items(s.items, [&](auto items) {
+      k_sort_scatter<items><<<(unsigned)s.tiles + extra, SORT_THREADS, 0, stream>>>(src, p * s.digit, s.digit, counts, totals, buf[p & 1], (int)s.tiles,
+                                                                                    fill);
+    });
     ORCA_LAUNCH_CHECK();
     src.pairs = buf[p & 1];
   }
@@ -1374,11 +1397,12 @@ ORCA_API int orca_embedding_backward_rows(const void* grad_out, int grad_dtype, 
   char* ws = (char*)workspace;
   const pair32* s = nullptr;
   if (int rc = sort_positions(idx64, idx32, n, num_rows, padding_idx, ws, l, fill_job{}, 0, &s, stream)) return rc;
-  const unsigned tiles = (unsigned)plan_sort(n, num_rows).tiles;
-  uint32_t* rank = (uint32_t*)(ws + l.rank);
-  k_rank_count<<<tiles, SORT_THREADS, 0, stream>>>(s, n, (uint32_t)num_rows, (uint32_t*)(ws + l.heads));
+  const sort_plan plan = plan_sort(n, num_rows);
+  const unsigned tiles = (unsigned)plan.tiles;
+  uint32_t *rank = (uint32_t*)(ws + l.rank), *heads = (uint32_t*)(ws + l.heads);
+  by_items(plan.items, [&](auto items) { k_rank_count<items><<<tiles, SORT_THREADS, 0, stream>>>(s, n, (uint32_t)num_rows, heads); });
   ORCA_LAUNCH_CHECK();
-  k_rank<<<tiles, SORT_THREADS, 0, stream>>>(s, n, (uint32_t)num_rows, (const uint32_t*)(ws + l.heads), rank, ids, count);
+  by_items(plan.items, [&](auto items) { k_rank<items><<<tiles, SORT_THREADS, 0, stream>>>(s, n, (uint32_t)num_rows, heads, rank, ids, count); });
   ORCA_LAUNCH_CHECK();
   seg_args a{grad_out, ld_grad, n, width, s, rank, rows, (float*)(ws + l.part), (int)width, 0, 0, window_of(n, width), 0, (uint32_t)num_rows, scale};
   return by_types(grad_dtype, rows_dtype, [&](auto gi, auto go) { return launch_sums<decltype(gi), decltype(go)>(a, false, stream); });
