@@ -556,3 +556,21 @@ def test_autograd_captured(ops):
     torch.cuda.synchronize()
     check_grad(grad, wgt, ids, vocab, 0.5, 0)
     assert torch.equal(grad, ops.embedding_backward(wgt, ids, vocab, 0.5, 0)), f"replay {r}"
+
+
+@pytest.mark.parametrize("n", [8193, 20001, 70000, 131072, 131073])
+@pytest.mark.parametrize("vocab", [1, 100, 1 << 14, 400_000, 4_000_003, 10_000_001, (1 << 31) - 2])
+def test_long_lists_and_row_numbers(ops, n, vocab):
+  """every number of passes, digit widths, and one to four pairs per thread: half the ids are hubs"""
+  g = torch.Generator().manual_seed(n + vocab % 1000)
+  ids = torch.where(torch.rand(n, generator=g) < 0.5, torch.randint(0, vocab, (n,), generator=g), torch.randint(0, 9, (n,), generator=g) * 7919 % vocab)
+  ids[0], ids[1], ids[2] = vocab - 1, -1, vocab
+  grad = torch.randn(n, 3, generator=g)
+  rg = ops.embedding_backward_rows(grad.to(DEV), ids.to(DEV), vocab, padding_idx=7919 % vocab if vocab > 1 else None)
+  ok = (ids >= 0) & (ids < vocab) & ((ids != 7919 % vocab) | (vocab == 1))
+  u, inv = torch.unique(ids[ok], return_inverse=True)
+  k = int(rg.count)
+  assert k == u.numel() and torch.equal(rg.ids[:k].cpu(), u)
+  z = torch.zeros(k, 3, dtype=torch.float64)
+  G, S = z.clone().index_add_(0, inv, grad[ok].double()), z.index_add_(0, inv, grad[ok].double().abs())
+  assert bool(((rg.rows[:k].cpu().double() - G).abs() <= bound(G, S, torch.bincount(inv), torch.float32)).all())
