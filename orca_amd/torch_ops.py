@@ -7,7 +7,8 @@ the reference's training loop differentiates (train.py:225-226 loss.backward()):
                       encodings of :126,132 fused in (rows fetched by index from the feature tables)
   orca::gru_cell      nn.GRUCell of modules/memory_updater.py:86 (get_updated_memory :56-78 applies it to the rows
                       of the pending ids a batch reads and keeps them in the graph)
-  orca::embedding     a learned table's rows by id, scaled (no counterpart upstream, where every table is data)
+  orca::embedding     a learned table's rows by id, scaled (no counterpart upstream, where every table is data);
+                      orca::embedding_backward is its gradient, differentiable in turn
   orca::message_store / orca::history_push / orca::history_pull     state writes and reads that are detached
                       upstream (tgn_model.py:172-191, history.py:32-40 run under no_grad)
 
@@ -225,26 +226,73 @@ _lib.register_autograd("orca::history_pull_pushed", _hpp_backward, setup_context
 
 
 # ---- a learned table: lookup with its gradient ------------------------------------------------------------------
-@_lib.custom_op("orca::embedding", mutates_args=())
-def embedding(table: Tensor, ids: Tensor, scale: float, padding_idx: int) -> Tensor:
+# Both directions are ops, each the other's derivative, so that a gradient of the gradient (create_graph=True) is there to any
+# order.  They are defined with their own autograd kernels: what custom_op registers lets the tangent of a table that does not
+# require a gradient go without a word.
+_table = _lib.Library("orca", "FRAGMENT")
+_table.define("embedding(Tensor table, Tensor ids, float scale, int padding_idx) -> Tensor")
+_table.define("embedding_backward(Tensor grad_out, Tensor ids, int num_rows, float scale, int padding_idx) -> Tensor")
+
+
+def _embedding(table, ids, scale, padding_idx):
   """scale * table[ids]; the row of padding_idx (negative: none) reads like any other and gets no gradient.  (A captured
   backward pass: as anywhere in torch, no eager graph of the same leaves may be alive.)"""
   return ops.embedding(table, ids, scale)
 
 
-def _embedding_setup(ctx, inputs, output):
-  table, ids, ctx.scale, ctx.padding_idx = inputs
-  ctx.num_rows = table.shape[0]
-  ctx.save_for_backward(ids)
+def _embedding_backward(grad_out, ids, num_rows, scale, padding_idx):
+  """the gradient of embedding for its table, dense"""
+  return ops.embedding_backward(grad_out, ids, num_rows, scale, padding_idx)
 
 
-def _embedding_backward(ctx, g_out):
-  ids, = ctx.saved_tensors
-  return ops.embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx), None, None, None
+_table.impl("embedding", _embedding, "CompositeExplicitAutograd")
+_table.impl("embedding_backward", _embedding_backward, "CompositeExplicitAutograd")
 
 
-_lib.register_autograd("orca::embedding", _embedding_backward, setup_context=_embedding_setup)
+class _Embedding(torch.autograd.Function):
+  @staticmethod
+  def forward(ctx, table, ids, scale, padding_idx):
+    ctx.num_rows, ctx.scale, ctx.padding_idx = table.shape[0], scale, padding_idx
+    ctx.save_for_backward(ids)
+    with torch._C._AutoDispatchBelowAutograd():
+      return torch.ops.orca.embedding(table, ids, scale, padding_idx)
+
+  @staticmethod
+  def backward(ctx, g_out):
+    ids, = ctx.saved_tensors
+    return torch.ops.orca.embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx), None, None, None
+
+
+class _EmbeddingBackward(torch.autograd.Function):
+  @staticmethod
+  def forward(ctx, grad_out, ids, num_rows, scale, padding_idx):
+    ctx.scale, ctx.padding_idx = scale, padding_idx
+    ctx.save_for_backward(ids)
+    with torch._C._AutoDispatchBelowAutograd():
+      return torch.ops.orca.embedding_backward(grad_out, ids, num_rows, scale, padding_idx)
+
+  @staticmethod
+  def backward(ctx, g_table):
+    ids, = ctx.saved_tensors
+    if ctx.padding_idx >= 0:          # the padding id's rows were not used: an id outside the table reads as zeros
+      ids = torch.where(ids == ctx.padding_idx, -1, ids)
+    return torch.ops.orca.embedding(g_table, ids, ctx.scale, -1), None, None, None, None
+
+
+def _table_autograd(name, function):
+  def kernel(x, *args):
+    if torch.autograd.forward_ad.unpack_dual(x).tangent is not None:
+      raise NotImplementedError(f"orca::{name} has no forward-mode derivative")
+    if torch.is_grad_enabled() and x.requires_grad:
+      return function.apply(x, *args)
+    with torch._C._AutoDispatchBelowAutograd():
+      return getattr(torch.ops.orca, name)(x, *args)
+  _table.impl(name, kernel, "Autograd")
+
+
+_table_autograd("embedding", _Embedding)
+_table_autograd("embedding_backward", _EmbeddingBackward)
 
 
 OPS = ("sample_recent", "sample_uniform", "tgat_dense", "tgat_gather", "gru_cell", "message_store", "history_push",
-       "history_pull", "history_pull_pushed", "embedding")
+       "history_pull", "history_pull_pushed", "embedding", "embedding_backward")
