@@ -419,7 +419,7 @@ int orca_decoder_train(const float* emb, int64_t bs, const float* fc1_w, const f
 /* out[p, :] = scale * table[ids[p], :], computed in fp32 and rounded once to the table's type (ORCA_F32 / BF16 / F16).
  * table [n_rows, width] with rows `ld` elements apart, ids int64 or int32 (exactly one list non-null), out [n, width]
  * without gaps.  An id outside [0, n_rows) reads as a row of zeros.  No alignment beyond the element's is needed;
- * 1 <= width <= 65536. */
+ * 1 <= width <= 65536; the output has under 2^34 pieces of 16 bytes (of one element where a row is shorter). */
 int orca_embedding_forward(const void* table, int dtype, int64_t n_rows, int64_t width, int64_t ld, const int64_t* idx64,
                            const int32_t* idx32, int64_t n, float scale, void* out, void* stream);
 /* The gradient of that lookup for the table: grad_table[v, :] = scale * sum over {p : ids[p] = v} of grad_out[p, :], zeros
@@ -427,7 +427,8 @@ int orca_embedding_forward(const void* table, int dtype, int64_t n_rows, int64_t
  * Ids outside [0, num_rows) and the id padding_idx (negative: none) contribute nothing; their rows of grad_out are never
  * used.  grad_out [n, width] with rows ld_grad elements apart (0: every row is the same one); grad_table's rows lie
  * ld_table >= width elements apart, its type is grad_dtype or ORCA_F32.  Sums are fp32 in an order that (id, position)
- * alone decides (the positions are sorted by id): the same call gives the same bits.  n and num_rows under 2^31 - 1.
+ * alone decides (the positions are sorted by id): the same call gives the same bits.  n and num_rows under 2^31 - 1, and
+ * n * width under 2^39.
  * workspace: orca_embedding_backward_workspace_bytes(n, width, num_rows) bytes (-1: unsupported sizes), 16-byte aligned,
  * contents irrelevant. */
 int64_t orca_embedding_backward_workspace_bytes(int64_t n, int64_t width, int64_t num_rows);

@@ -28,19 +28,21 @@ int adam_groups(int n, float* const* params, const float* const* grads, float* c
                "orca_adam_step: bad arguments");
   for (int i0 = 0; i0 < n; i0 += ADAM_MAX) {
     AdamGroup grp{};
-    int first = 0, k = 0;
+    int64_t first = 0;
+    int k = 0;
     for (int i = i0; i < n && i < i0 + ADAM_MAX; ++i) {
       if (sizes[i] <= 0) continue;
       ORCA_REQUIRE(params[i] && grads[i] && exp_avg[i] && exp_avg_sq[i], "orca_adam_step: null tensor %d", i);
       ORCA_REQUIRE(sizes[i] < (1LL << 40), "orca_adam_step: tensor %d too large", i);
-      grp.first[k] = first;
+      grp.first[k] = (int)first;
       grp.p[k] = params[i]; grp.g[k] = grads[i]; grp.m[k] = exp_avg[i]; grp.v[k] = exp_avg_sq[i]; grp.size[k] = sizes[i];
-      first += (int)ceil_div64(sizes[i], 1024);
+      first += ceil_div64(sizes[i], 1024);
+      ORCA_REQUIRE(first < (1 << 24), "orca_adam_step: too many elements for one call");      // (a launch has under 2^32 threads)
       ++k;
     }
     if (k == 0) continue;
     grp.n = k;
-    grp.first[k] = first;
+    grp.first[k] = (int)first;
     launch(grp, (unsigned)first);
   }
   ORCA_LAUNCH_CHECK();

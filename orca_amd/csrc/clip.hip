@@ -26,6 +26,7 @@ constexpr int GRID = 2048, LONG_GRID = 1024, PARTS = 2048, LONG_PARTS = 8192;
 // Pieces of a workgroup of k_clip on a long list in place: when the coefficient is 1 they all only come and go (500 MB of fp32 with one
 // piece, four, sixteen: 107, 91, 87 us; with a coefficient below 1 233, 226, 238).
 constexpr int IN_PLACE_PIECES = 4;
+constexpr unsigned MOST_BLOCKS = 1 << 22;       // (a launch has under 2^32 threads; more pieces go round)
 constexpr int SPARSE_MAX = 4;         // row-sparse tensors per launch
 
 struct sparse_grad {
@@ -335,7 +336,8 @@ int clip(const host_list& h, void* const* flat, const float* coef, const double*
       for (int k = 0; k < 3; ++k) list.flat[k] = (char*)flat[k] + to[k] * (k == ORCA_F32 ? 4 : 2);
     take<L, FLAT>(h, &i, to, &list);
     if (list.n == 0) continue;
-    const unsigned pieces = (unsigned)list.first[list.n], grid = std::min<unsigned>(pieces, GRID), many = FLAT ? pieces : (pieces - 1) / IN_PLACE_PIECES + 1;
+    const unsigned pieces = (unsigned)list.first[list.n], grid = std::min<unsigned>(pieces, GRID),
+                   many = std::min(FLAT ? pieces : (pieces - 1) / IN_PLACE_PIECES + 1, MOST_BLOCKS);
     if (h.piece == LONG_PIECE) k_clip<LONG_PIECE, true, L, FLAT><<<many, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
     else if (h.piece == PIECE) k_clip<PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);
     else k_clip<SMALL_PIECE, false, L, FLAT><<<grid, 256, 0, stream>>>(list, coef, part, parts, max_norm, norm);

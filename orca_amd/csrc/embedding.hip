@@ -39,6 +39,8 @@ bool past_zeros(int64_t bytes) { return bytes >= 384 * MB; }
 bool past_gradient(int64_t bytes) { return bytes >= 128 * MB; }
 
 constexpr int64_t MAX_WIDTH = 65536;      // x * C of the division below stays under 2^32
+// A launch has under 2^32 threads (the runtime's limit for blocks * threads).
+bool fits_launch(int64_t blocks, int threads) { return blocks * threads < (1LL << 32); }
 
 // ---- lookup ----------------------------------------------------------------------------------------------------------
 // The output is a list of n * C chunks of 16 bytes; the last chunk of a row starts at width - VEC, so that every access is
@@ -90,7 +92,7 @@ template <class T, int VEC, class I>
 int launch_embedding(const void* table, int64_t n_rows, int64_t width, int64_t ld, const I* ids, int64_t n, float scale, void* out,
                      hipStream_t stream) {
   const int64_t C = ceil_div64(width, VEC), total = n * C, blocks = ceil_div64(total, 256 * LOOK_U);
-  ORCA_REQUIRE(blocks < (1LL << 31), "orca_embedding_forward: %lld rows of %lld values are too many for one call", (long long)n, (long long)width);
+  ORCA_REQUIRE(fits_launch(blocks, 256), "orca_embedding_forward: %lld rows of %lld values are too many for one call", (long long)n, (long long)width);
   const uint32_t magic = C == 1 ? 0 : (uint32_t)(((1ULL << 32) + C - 1) / C);
   auto* kernel = VEC > 1 && past_lookup(n * width * (int64_t)sizeof(T)) ? k_embedding<T, VEC, VEC != 1, I> : k_embedding<T, VEC, false, I>;
   kernel<<<(unsigned)blocks, 256, 0, stream>>>((const T*)table, n_rows, ld, ids, total, (int)width, (uint32_t)C, magic, scale, (T*)out);
@@ -1121,17 +1123,34 @@ work_layout layout(int64_t n, int64_t width, int64_t num_rows) {
   l.bytes = o;
   return l;
 }
+// teams of lanes over the columns, and the workgroups of the windows' sums and of their joins
+struct sums_grid { int chunks, log_l, col_blocks; int64_t blocks; };
+sums_grid segment_grid(int64_t n, int64_t width, int vec) {
+  sums_grid g;
+  g.chunks = (int)(width < vec ? width : ceil_div64(width, vec));
+  g.log_l = log_lanes(g.chunks, 8);
+  g.col_blocks = (int)ceil_div64(g.chunks, 1 << g.log_l);
+  g.blocks = ceil_div64(ceil_div64(n, window_of(n, width)), 256 >> g.log_l) * g.col_blocks;
+  return g;
+}
+sums_grid join_grid(int64_t n, int64_t width) {
+  sums_grid g;
+  g.chunks = (int)ceil_div64(width, 4);
+  g.log_l = log_lanes(g.chunks, 6);
+  g.col_blocks = (int)ceil_div64(g.chunks, 1 << g.log_l);
+  g.blocks = ceil_div64(ceil_div64(n, window_of(n, width)) - 1, JOIN_THREADS >> g.log_l) * g.col_blocks;
+  return g;
+}
 template <class TI, class TO, int VEC>
 int launch_sums_vec(seg_args a, bool accumulate, hipStream_t stream) {
-  a.chunks = VEC == 1 ? a.width : (a.width + VEC - 1) / VEC;
-  a.log_l = log_lanes(a.chunks, 8);
-  a.col_blocks = (int)ceil_div64(a.chunks, 1 << a.log_l);
-  const int64_t windows = ceil_div64(a.n, a.window), blocks = ceil_div64(windows, 256 >> a.log_l) * a.col_blocks;
-  ORCA_REQUIRE(blocks < (1LL << 31), "orca_embedding_backward: %lld ids of width %d are too many for one call", (long long)a.n, a.width);
+  const sums_grid grid = segment_grid(a.n, a.width, elems16<TI>);
+  a.chunks = grid.chunks;
+  a.log_l = grid.log_l;
+  a.col_blocks = grid.col_blocks;
   const bool past = VEC > 1 && past_gradient(a.n * a.width * (int64_t)sizeof(TI));
   auto* kernel = accumulate ? (past ? k_segment_sum<TI, TO, VEC, true, VEC != 1> : k_segment_sum<TI, TO, VEC, true, false>)
                             : (past ? k_segment_sum<TI, TO, VEC, false, VEC != 1> : k_segment_sum<TI, TO, VEC, false, false>);
-  kernel<<<(unsigned)blocks, 256, 0, stream>>>(a);
+  kernel<<<(unsigned)grid.blocks, 256, 0, stream>>>(a);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
@@ -1139,15 +1158,13 @@ template <class TI, class TO>
 int launch_sums(seg_args a, bool accumulate, hipStream_t stream) {
   constexpr int VEC = elems16<TI>;
   if (int rc = a.width >= VEC ? launch_sums_vec<TI, TO, VEC>(a, accumulate, stream) : launch_sums_vec<TI, TO, 1>(a, accumulate, stream)) return rc;
-  const int64_t windows = ceil_div64(a.n, a.window);
-  if (windows < 2) return ORCA_OK;
-  a.chunks = (a.width + 3) / 4;
-  a.log_l = log_lanes(a.chunks, 6);
-  a.col_blocks = (int)ceil_div64(a.chunks, 1 << a.log_l);
-  const int64_t blocks = ceil_div64(windows - 1, JOIN_THREADS >> a.log_l) * a.col_blocks;
-  ORCA_REQUIRE(blocks < (1LL << 31), "orca_embedding_backward: %lld ids of width %d are too many for one call", (long long)a.n, a.width);
-  if (accumulate) k_segment_join<TO, true><<<(unsigned)blocks, JOIN_THREADS, 0, stream>>>(a);
-  else k_segment_join<TO, false><<<(unsigned)blocks, JOIN_THREADS, 0, stream>>>(a);
+  const sums_grid grid = join_grid(a.n, a.width);
+  if (grid.blocks == 0) return ORCA_OK;          // (one window)
+  a.chunks = grid.chunks;
+  a.log_l = grid.log_l;
+  a.col_blocks = grid.col_blocks;
+  if (accumulate) k_segment_join<TO, true><<<(unsigned)grid.blocks, JOIN_THREADS, 0, stream>>>(a);
+  else k_segment_join<TO, false><<<(unsigned)grid.blocks, JOIN_THREADS, 0, stream>>>(a);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
@@ -1260,6 +1277,9 @@ int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, co
   if (n == 0) return ORCA_OK;
   ORCA_REQUIRE(g && (idx64 != nullptr) != (idx32 != nullptr), "%s: null gradient, or not exactly one list of ids", who);
   ORCA_REQUIRE(ld_g >= 0, "%s: negative row stride", who);
+  ORCA_REQUIRE(is_small(n, width) || (fits_launch(segment_grid(n, width, g_dtype == ORCA_F32 ? elems16<float> : elems16<__bf16>).blocks, 256) &&
+                                      fits_launch(join_grid(n, width).blocks, JOIN_THREADS)),
+               "%s: %lld ids of width %lld are too many for one call", who, (long long)n, (long long)width);
   ORCA_REQUIRE(((uintptr_t)workspace & 15) == 0, "%s: the workspace is not 16-byte aligned", who);
   ORCA_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(n, width, num_rows), "%s: the workspace holds %lld of %lld bytes", who,
                (long long)workspace_bytes, (long long)workspace_bytes_of(n, width, num_rows));
@@ -1267,11 +1287,14 @@ int check_gradient(const char* who, const void* g, int g_dtype, int64_t ld_g, co
 }
 
 // the pieces of a fill that launch `i` of `launches` takes, and the workgroups for them.  (Even shares: a million rows of 400 bytes 81 us;
-// 80 MB in the sort's launches and the rest ahead of the sums: 92; everything ahead of the sort: 100.)
+// 80 MB in the sort's launches and the rest ahead of the sums: 92; everything ahead of the sort: 100.)  At most FILL_BLOCKS of them, which
+// then go round: with the sort's tiles that stays within a launch (in a table with gaps every row is a piece).
+constexpr int64_t FILL_BLOCKS = 1 << 22;
+static_assert((FILL_BLOCKS + (1LL << 31) / (4 * SORT_THREADS)) * SORT_THREADS < (1LL << 32), "threads of a launch");
 unsigned fill_share(fill_job* f, int64_t pieces, int threads, int i, int launches) {
   f->from = pieces * i / launches;
   f->to = pieces * (i + 1) / launches;
-  return (unsigned)std::min<int64_t>(ceil_div64(f->to - f->from, threads / 256), 1 << 24);
+  return (unsigned)std::min<int64_t>(ceil_div64(f->to - f->from, threads / 256), FILL_BLOCKS);
 }
 int launch_fill(fill_job f, int64_t pieces, hipStream_t stream) {
   const unsigned blocks = fill_share(&f, pieces, 256, 0, 1);
