@@ -6,7 +6,6 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <algorithm>
@@ -75,10 +74,53 @@ void arguments(Py_ssize_t n, Py_ssize_t want) {
   if (n != want) refuse(PyExc_TypeError, "expected ", want, " arguments, got ", n);
 }
 
+// The bytes of a strided tensor: runs of `run` bytes, repeated along `outer` (stride in bytes ascending, size at least 2).
+struct region {
+  const char* p;
+  int64_t run;
+  c10::SmallVector<std::pair<int64_t, int64_t>, 4> outer;
+  const char* end() const {
+    int64_t n = run;
+    for (const auto& d : outer) n += d.first * (d.second - 1);
+    return p + n;
+  }
+};
+region region_of(const at::Tensor& t) {
+  region r{(const char*)t.const_data_ptr(), t.numel() ? (int64_t)t.element_size() : 0, {}};
+  if (!r.run) return r;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d)) r.outer.emplace_back(t.stride(d) * r.run, t.size(d));
+  std::sort(r.outer.begin(), r.outer.end());
+  while (!r.outer.empty() && r.outer.front().first <= r.run) {        // (no gap between the repetitions)
+    r.run += r.outer.front().first * (r.outer.front().second - 1);
+    r.outer.erase(r.outer.begin());
+  }
+  return r;
+}
+// Whether they share a byte.  Views that interleave (column blocks of one matrix) do not.
+bool meet(const region& a, const region& b) {
+  if (!a.run || !b.run || a.end() <= b.p || b.end() <= a.p) return false;
+  if (a.outer.empty() && b.outer.empty()) return true;
+  if (a.outer.size() == 1 && b.outer.size() == 1 && a.outer[0].first == b.outer[0].first) {
+    // a's run i lies at `at` of the pitch behind the beginning of b's run i + k: it may reach that one and the next
+    const int64_t pitch = a.outer[0].first, d = a.p - b.p, k = d >= 0 ? d / pitch : -((-d + pitch - 1) / pitch), at = d - k * pitch;
+    auto both = [&](int64_t k) { return std::max<int64_t>(0, -k) <= std::min(a.outer[0].second - 1, b.outer[0].second - 1 - k); };
+    return (at < b.run && both(k)) || (at + a.run > pitch && both(k + 1));
+  }
+  const bool left = !a.outer.empty() && (b.outer.empty() || a.end() - a.p >= b.end() - b.p);        // halve the longer one
+  region x = left ? a : b, y = x;
+  auto& [stride, size] = x.outer.back();
+  y.p += stride * (size / 2);
+  y.outer.back().second -= size / 2;
+  size /= 2;
+  if (size == 1) x.outer.pop_back();
+  if (y.outer.back().second == 1) y.outer.pop_back();
+  return left ? meet(x, b) || meet(y, b) : meet(a, x) || meet(a, y);
+}
+
 // an output that shares memory with an input
 void apart(const at::Tensor& out, const at::Tensor& in, const char* who, const char* what) {
-  const at::MemOverlapStatus s = at::get_overlap_status(out, in);
-  if (s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial) refuse(PyExc_ValueError, who, ": out overlaps ", what);
+  if (meet(region_of(out), region_of(in))) refuse(PyExc_ValueError, who, ": out overlaps ", what);
 }
 
 // embedding(table, ids, scale, out)
