@@ -147,6 +147,7 @@ PyObject* embedding(PyObject* const* a, Py_ssize_t n) {
     if (c != code || out.device() != dev || !out.is_contiguous() || out.sizes() != at::IntArrayRef(shape))
       refuse(PyExc_ValueError, "embedding: out must be a contiguous ", table.scalar_type(), " tensor of shape ", at::IntArrayRef(shape), " on ", dev);
     apart(out, table, "embedding", "the table");
+    apart(out, ids.t, "embedding", "the ids");
   }
   check(embedding_forward(table.const_data_ptr(), code, table.size(0), width, table.stride(0), ids.i64, ids.i32, ids.t.numel(), (float)scale,
                           out.data_ptr(), stream_of(dev)),
@@ -217,6 +218,7 @@ PyObject* embedding_backward(PyObject* const* a, Py_ssize_t n) {
       refuse(PyExc_ValueError, "embedding_backward: out must be a tensor of shape [", b.num_rows, ", ", b.width, "] on ", b.dev,
              " of the gradient's type or float32, whose rows are contiguous and do not overlap");
     apart(out, b.g, who, "grad_out");
+    apart(out, b.ids.t, who, "the ids");
   }
   check(embedding_backward_c(b.g.const_data_ptr(), b.code, b.n ? b.g.stride(0) : 0, b.ids.i64, b.ids.i32, b.n, b.width, b.num_rows, b.padding, b.scale,
                              accumulate, out.data_ptr(), type, out.stride(0), ws.data_ptr(), bytes, stream_of(b.dev)),
@@ -252,8 +254,13 @@ PyObject* embedding_backward_rows(PyObject* const* a, Py_ssize_t n) {
         (a[6] != Py_None && type_of(a[6], b, who) != type))
       refuse(PyExc_ValueError, who, ": out must be contiguous int64 [", b.n, "], gradient-typed or float32 [", b.n, ", ", b.width,
              "] and int32 [1] tensors on ", b.dev);
-    apart(rows, b.g, who, "grad_out");
-    apart(ids, b.ids.t, who, "the ids");
+    for (const at::Tensor* o : {&ids, &rows, &count}) {
+      apart(*o, b.g, who, "grad_out");
+      apart(*o, b.ids.t, who, "the ids");
+    }
+    apart(ids, rows, who, "itself (ids and rows)");
+    apart(ids, count, who, "itself (ids and count)");
+    apart(rows, count, who, "itself (rows and count)");
   }
   check(embedding_backward_rows_c(b.g.const_data_ptr(), b.code, b.n ? b.g.stride(0) : 0, b.ids.i64, b.ids.i32, b.n, b.width, b.num_rows, b.padding,
                                   b.scale, (int64_t*)ids.data_ptr(), rows.data_ptr(), type, (int32_t*)count.data_ptr(), ws.data_ptr(), bytes,

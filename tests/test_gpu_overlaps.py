@@ -41,3 +41,37 @@ def test_strided_gradients(ops):
   for out in (buf[:5, 8:16], buf[4:9, :8], buf[7:, 16:]):                  # other columns, other rows
     assert torch.equal(ops.embedding_backward(buf[:4, :8], ids, 5, out=out), want)
   assert torch.equal(buf[:4, :8], keep[:4, :8])
+
+
+def test_ids_in_the_output(ops):
+  """the ids and the output in one storage, seen as different types"""
+  buf = torch.zeros(64, dtype=torch.int64, device=DEV)
+  buf[:4] = torch.tensor([1, 0, 3, 1], device=DEV)
+  f = buf.view(torch.float32)                                    # 128 values: the ids are the first 8
+  table, grad = torch.randn(5, 8, device=DEV), torch.randn(4, 8, device=DEV)
+  for ids, n in ((buf[:4], 8), (buf.view(torch.int32)[:8:2], 8)):          # (the second is copied: its copy shares nothing)
+    if ids.dtype == torch.int64:
+      with pytest.raises(ValueError, match="overlaps the ids"):
+        ops.embedding(table, ids, out=f[n - 1:n + 31].view(4, 8))
+      with pytest.raises(ValueError, match="overlaps the ids"):
+        ops.embedding_backward(grad, ids, 5, out=f[n - 2:n + 38].view(5, 8))
+    assert torch.equal(ops.embedding(table, ids, out=f[n:n + 32].view(4, 8)), table[ids.long()])
+    assert torch.equal(ops.embedding_backward(grad, ids, 5, out=f[n:n + 40].view(5, 8)), ops.embedding_backward(grad, ids.clone(), 5))
+  assert buf[:4].tolist() == [1, 0, 3, 1]
+
+
+def test_row_outputs_in_one_storage(ops):
+  ids, grad = torch.tensor([1, 0, 3, 1], device=DEV), torch.randn(4, 8, device=DEV)
+  buf = torch.zeros(64, dtype=torch.int64, device=DEV)
+  f, i = buf.view(torch.float32), buf.view(torch.int32)
+  out = lambda a, r, c: (buf[a:a + 4], f[r:r + 32].view(4, 8), i[c:c + 1])
+  for bad in (out(0, 7, 50), out(0, 8, 7), out(0, 8, 39), out(3, 0, 50)):
+    with pytest.raises(ValueError, match="overlaps"):
+      ops.embedding_backward_rows(grad, ids, 5, out=bad)
+  for bad in ((buf[:4], f[8:40].view(4, 8), grad.view(torch.int32)[3, 7:]), (buf[:4], f[8:40].view(4, 8), ids.view(torch.int32)[1:2]),
+              (grad.view(torch.int64).view(-1)[12:], f[8:40].view(4, 8), i[60:61]), (buf[:4], ids.view(torch.float32)[:0].expand(0), i[60:61])):
+    with pytest.raises(ValueError):
+      ops.embedding_backward_rows(grad, ids, 5, out=bad)
+  assert not bool(buf.any()) and ids.tolist() == [1, 0, 3, 1]
+  got, want = ops.embedding_backward_rows(grad, ids, 5, out=out(0, 8, 40)), ops.embedding_backward_rows(grad, ids, 5)
+  assert int(got.count) == int(want.count) == 3 and torch.equal(got.ids[:3], want.ids[:3]) and torch.equal(got.rows[:3], want.rows[:3])
