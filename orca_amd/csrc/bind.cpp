@@ -281,7 +281,8 @@ struct grad_arrays {
   std::vector<uint8_t> types;
   std::vector<const int32_t*> rows;           // empty: none is row-sparse
   std::vector<int32_t> widths;
-  std::vector<std::pair<at::Tensor, at::Tensor>> copies;        // (contiguous copy, the caller's tensor)
+  struct copy { at::Tensor made, of; size_t at; };
+  std::vector<copy> copies;                   // contiguous copies, the caller's tensors, their places in the list
   c10::Device dev{at::kCUDA, (c10::DeviceIndex)-1};
 };
 grad_arrays grads_of(PyObject* list, const char* who) {
@@ -318,8 +319,8 @@ grad_arrays grads_of(PyObject* list, const char* who) {
     if (t.is_contiguous()) {
       r.data.push_back(t.data_ptr());
     } else {
-      r.copies.emplace_back(t.contiguous(), t);
-      r.data.push_back(r.copies.back().first.data_ptr());
+      r.copies.push_back({t.contiguous(), t, r.data.size()});
+      r.data.push_back(r.copies.back().made.data_ptr());
     }
     r.sizes.push_back(t.numel());
     r.types.push_back((uint8_t)code);
@@ -353,20 +354,41 @@ PyObject* grad_norm(PyObject* const* a, Py_ssize_t n) {
   return r;
 }
 
-// the bytes of the list's tensors: where they begin, where they end
-typedef std::pair<const char*, const char*> span;
-span span_of(const void* p, int64_t n, int code) { return {(const char*)p, (const char*)p + n * (code == ORCA_F32 ? 4 : 2)}; }
+// the bytes of the list's tensors, in their callers' storage: contiguous ones as they are, the others by their strides
+struct span {
+  const char *first, *last;           // from .. up to
+  const at::Tensor* strided;          // null: contiguous
+  region bytes() const { return strided ? region_of(*strided) : region{first, last - first, {}}; }
+};
+span span_of(const void* p, int64_t n, int code) { return {(const char*)p, (const char*)p + n * (code == ORCA_F32 ? 4 : 2), nullptr}; }
 std::vector<span> spans_of(const grad_arrays& g) {
   std::vector<span> s;
   s.reserve(g.data.size());
-  for (size_t i = 0; i < g.data.size(); ++i)
-    if (g.sizes[i]) s.push_back(span_of(g.data[i], g.sizes[i], g.types[i]));
+  size_t next = 0;
+  for (size_t i = 0; i < g.data.size(); ++i) {
+    const at::Tensor* t = next < g.copies.size() && g.copies[next].at == i ? &g.copies[next++].of : nullptr;
+    if (!g.sizes[i]) continue;
+    if (t) {
+      const region r = region_of(*t);
+      s.push_back({r.p, r.end(), t});
+    } else {
+      s.push_back(span_of(g.data[i], g.sizes[i], g.types[i]));
+    }
+  }
   return s;
 }
+bool meet(const span& a, const span& b) {
+  return a.first < b.last && b.first < a.last && ((!a.strided && !b.strided) || meet(a.bytes(), b.bytes()));
+}
 void apart_in_list(std::vector<span> s, const char* who) {
-  std::sort(s.begin(), s.end());
-  for (size_t i = 1; i < s.size(); ++i)
-    if (s[i].first < s[i - 1].second) refuse(PyExc_ValueError, who, ": a tensor is in the list twice, or two of them overlap");
+  std::sort(s.begin(), s.end(), [](const span& a, const span& b) { return a.first < b.first; });
+  std::vector<const span*> open;                // those that reach past the beginning of the next one
+  for (const span& x : s) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const span* o) { return o->last <= x.first; }), open.end());
+    for (const span* o : open)
+      if (meet(*o, x)) refuse(PyExc_ValueError, who, ": a tensor is in the list twice, or two of them overlap");
+    open.push_back(&x);
+  }
 }
 
 // clip_grad_norm(list, max_norm, flat buffers or None) -> norm
@@ -380,8 +402,8 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
   if (a[2] == Py_None) {
     apart_in_list(spans_of(g), who);
     for (const auto& c : g.copies)
-      for (int64_t d = 0; d < c.second.dim(); ++d)
-        if (c.second.stride(d) == 0 && c.second.size(d) > 1) refuse(PyExc_ValueError, who, ": an expanded tensor cannot be clipped in place");
+      for (int64_t d = 0; d < c.of.dim(); ++d)
+        if (c.of.stride(d) == 0 && c.of.size(d) > 1) refuse(PyExc_ValueError, who, ": an expanded tensor cannot be clipped in place");
   } else {
     if (!PyList_Check(a[2])) refuse(PyExc_TypeError, who, ": flat must be a list of tensors");
     std::vector<int> order;                       // the types as they first appear
@@ -402,11 +424,9 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
       flat[code] = f.data_ptr();
       if (f.numel()) written.push_back(span_of(f.data_ptr(), f.numel(), code));
     }
-    for (size_t i = 0; i < g.data.size(); ++i) {
-      const span r = span_of(g.data[i], g.sizes[i], g.types[i]);
+    for (const span& r : spans_of(g))
       for (const span& w : written)
-        if (w.first < r.second && r.first < w.second) refuse(PyExc_ValueError, who, ": a flat buffer overlaps a gradient");
-    }
+        if (meet(w, r)) refuse(PyExc_ValueError, who, ": a flat buffer overlaps a gradient");
     apart_in_list(std::move(written), who);
   }
   const auto opt = at::TensorOptions(g.dev).dtype(at::kFloat);
@@ -415,7 +435,7 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
                      a[2] == Py_None ? nullptr : flat, norm.data_ptr<float>(), ws.data_ptr(), stream_of(g.dev)),
         "orca_clip_grads");
   if (a[2] == Py_None)
-    for (const auto& c : g.copies) c.second.detach().copy_(c.first);
+    for (const auto& c : g.copies) c.of.detach().copy_(c.made);
   return THPVariable_Wrap(norm);
 }
 
