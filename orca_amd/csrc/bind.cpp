@@ -202,6 +202,7 @@ PyObject* embedding_backward(PyObject* const* a, Py_ssize_t n) {
   const char* who = "embedding_backward";
   const backward_args b = backward_of(a, who);
   const int accumulate = PyObject_IsTrue(a[6]);
+  if (accumulate < 0) throw python_error();
   const c10::DeviceGuard guard(b.dev);
   int64_t bytes;
   const at::Tensor ws = workspace_of(b, &bytes, who);

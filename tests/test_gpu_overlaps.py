@@ -75,3 +75,16 @@ def test_row_outputs_in_one_storage(ops):
   assert not bool(buf.any()) and ids.tolist() == [1, 0, 3, 1]
   got, want = ops.embedding_backward_rows(grad, ids, 5, out=out(0, 8, 40)), ops.embedding_backward_rows(grad, ids, 5)
   assert int(got.count) == int(want.count) == 3 and torch.equal(got.ids[:3], want.ids[:3]) and torch.equal(got.rows[:3], want.rows[:3])
+
+
+def test_a_flag_without_a_truth_value(ops):
+  """what raises when it is asked for its truth value raises out of the call, and nothing is written"""
+  class Odd:
+    def __bool__(self):
+      raise KeyError("no truth value")
+  ids, grad, out = torch.tensor([1, 0], device=DEV), torch.ones(2, 4, device=DEV), torch.full((3, 4), 7.0, device=DEV)
+  with pytest.raises(KeyError, match="no truth value"):
+    ops.embedding_backward(grad, ids, 3, out=out, accumulate=Odd())
+  with pytest.raises(RuntimeError):
+    ops.embedding_backward(grad, ids, 3, out=out, accumulate=torch.zeros(2))
+  assert bool((out == 7).all())
