@@ -74,6 +74,12 @@ void arguments(Py_ssize_t n, Py_ssize_t want) {
   if (n != want) refuse(PyExc_TypeError, "expected ", want, " arguments, got ", n);
 }
 
+// A caller's tensor that the kernels write: autograd has to see it (it refuses a backward pass through a value that was saved and then
+// changed).  Inference tensors have no version.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // The bytes of a strided tensor: runs of `run` bytes, repeated along `outer` (stride in bytes ascending, size at least 2).
 struct region {
   const char* p;
@@ -152,6 +158,7 @@ PyObject* embedding(PyObject* const* a, Py_ssize_t n) {
   check(embedding_forward(table.const_data_ptr(), code, table.size(0), width, table.stride(0), ids.i64, ids.i32, ids.t.numel(), (float)scale,
                           out.data_ptr(), stream_of(dev)),
         "orca_embedding_forward");
+  if (a[3] != Py_None) written(out);
   return THPVariable_Wrap(out);
 }
 
@@ -224,6 +231,7 @@ PyObject* embedding_backward(PyObject* const* a, Py_ssize_t n) {
   check(embedding_backward_c(b.g.const_data_ptr(), b.code, b.n ? b.g.stride(0) : 0, b.ids.i64, b.ids.i32, b.n, b.width, b.num_rows, b.padding, b.scale,
                              accumulate, out.data_ptr(), type, out.stride(0), ws.data_ptr(), bytes, stream_of(b.dev)),
         "orca_embedding_backward");
+  if (a[5] != Py_None) written(out);
   return THPVariable_Wrap(out);
 }
 
@@ -267,6 +275,8 @@ PyObject* embedding_backward_rows(PyObject* const* a, Py_ssize_t n) {
                                   b.scale, (int64_t*)ids.data_ptr(), rows.data_ptr(), type, (int32_t*)count.data_ptr(), ws.data_ptr(), bytes,
                                   stream_of(b.dev)),
         "orca_embedding_backward_rows");
+  if (a[5] != Py_None)
+    for (const at::Tensor* o : {&ids, &rows, &count}) written(*o);
   PyObject* r = PyTuple_New(3);
   if (!r) throw python_error();
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(ids));
@@ -278,12 +288,12 @@ PyObject* embedding_backward_rows(PyObject* const* a, Py_ssize_t n) {
 // a list of tensors, RowGrads and Nones as the host arrays of orca_grad_norm / orca_clip_grads
 struct grad_arrays {
   std::vector<void*> data;
+  std::vector<const at::Tensor*> tensors;     // the list's own
   std::vector<int64_t> sizes;
   std::vector<uint8_t> types;
   std::vector<const int32_t*> rows;           // empty: none is row-sparse
   std::vector<int32_t> widths;
-  struct copy { at::Tensor made, of; size_t at; };
-  std::vector<copy> copies;                   // contiguous copies, the caller's tensors, their places in the list
+  std::vector<std::pair<at::Tensor, size_t>> copies;        // contiguous copies, their places in the list
   c10::Device dev{at::kCUDA, (c10::DeviceIndex)-1};
 };
 grad_arrays grads_of(PyObject* list, const char* who) {
@@ -291,6 +301,7 @@ grad_arrays grads_of(PyObject* list, const char* who) {
   grad_arrays r;
   const Py_ssize_t n = PyList_GET_SIZE(list);
   r.data.reserve(n);
+  r.tensors.reserve(n);
   r.sizes.reserve(n);
   r.types.reserve(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -320,9 +331,10 @@ grad_arrays grads_of(PyObject* list, const char* who) {
     if (t.is_contiguous()) {
       r.data.push_back(t.data_ptr());
     } else {
-      r.copies.push_back({t.contiguous(), t, r.data.size()});
-      r.data.push_back(r.copies.back().made.data_ptr());
+      r.copies.emplace_back(t.contiguous(), r.data.size());
+      r.data.push_back(r.copies.back().first.data_ptr());
     }
+    r.tensors.push_back(&t);
     r.sizes.push_back(t.numel());
     r.types.push_back((uint8_t)code);
   }
@@ -367,11 +379,12 @@ std::vector<span> spans_of(const grad_arrays& g) {
   s.reserve(g.data.size());
   size_t next = 0;
   for (size_t i = 0; i < g.data.size(); ++i) {
-    const at::Tensor* t = next < g.copies.size() && g.copies[next].at == i ? &g.copies[next++].of : nullptr;
+    const bool copied = next < g.copies.size() && g.copies[next].second == i;
+    next += copied;
     if (!g.sizes[i]) continue;
-    if (t) {
-      const region r = region_of(*t);
-      s.push_back({r.p, r.end(), t});
+    if (copied) {
+      const region r = region_of(*g.tensors[i]);
+      s.push_back({r.p, r.end(), g.tensors[i]});
     } else {
       s.push_back(span_of(g.data[i], g.sizes[i], g.types[i]));
     }
@@ -403,8 +416,8 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
   if (a[2] == Py_None) {
     apart_in_list(spans_of(g), who);
     for (const auto& c : g.copies)
-      for (int64_t d = 0; d < c.of.dim(); ++d)
-        if (c.of.stride(d) == 0 && c.of.size(d) > 1) refuse(PyExc_ValueError, who, ": an expanded tensor cannot be clipped in place");
+      for (int64_t d = 0; d < g.tensors[c.second]->dim(); ++d)
+        if (g.tensors[c.second]->stride(d) == 0 && g.tensors[c.second]->size(d) > 1) refuse(PyExc_ValueError, who, ": an expanded tensor cannot be clipped in place");
   } else {
     if (!PyList_Check(a[2])) refuse(PyExc_TypeError, who, ": flat must be a list of tensors");
     std::vector<int> order;                       // the types as they first appear
@@ -435,8 +448,12 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
   check(clip_grads_c((int)g.data.size(), g.data.data(), g.sizes.data(), g.types.data(), g.rows.empty() ? nullptr : g.rows.data(), g.widths.data(), max_norm,
                      a[2] == Py_None ? nullptr : flat, norm.data_ptr<float>(), ws.data_ptr(), stream_of(g.dev)),
         "orca_clip_grads");
-  if (a[2] == Py_None)
-    for (const auto& c : g.copies) c.of.detach().copy_(c.made);
+  if (a[2] == Py_None) {
+    for (const auto& c : g.copies) g.tensors[c.second]->detach().copy_(c.first);
+    for (const at::Tensor* t : g.tensors) written(*t);
+  } else {
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(a[2]); ++k) written(THPVariable_Unpack(PyList_GET_ITEM(a[2], k)));
+  }
   return THPVariable_Wrap(norm);
 }
 
