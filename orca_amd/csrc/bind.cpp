@@ -42,6 +42,12 @@ const at::Tensor& elements(PyObject* o, const char* what, int* code) {
   if (!t.is_cuda()) refuse(orca_error, what, ": expected a tensor on the HIP device (no CPU fallback)");
   return t;
 }
+// one whose memory holds its values (the imaginary part of a conjugated tensor is a view that torch negates when it is read)
+const at::Tensor& plain_elements(PyObject* o, const char* what, int* code) {
+  const at::Tensor& t = elements(o, what, code);
+  if (t.is_neg()) refuse(PyExc_ValueError, what, ": a lazily negated view (resolve_neg() makes a tensor of it)");
+  return t;
+}
 struct id_list {
   at::Tensor t;
   const int64_t* i64 = nullptr;
@@ -133,7 +139,7 @@ void apart(const at::Tensor& out, const at::Tensor& in, const char* who, const c
 PyObject* embedding(PyObject* const* a, Py_ssize_t n) {
   arguments(n, 4);
   int code;
-  const at::Tensor& table = elements(a[0], "embedding table", &code);
+  const at::Tensor& table = plain_elements(a[0], "embedding table", &code);
   if (table.dim() != 2) refuse(PyExc_ValueError, "embedding: table has shape ", table.sizes(), ", expected [n_rows, width]");
   const c10::Device dev = table.device();
   const id_list ids = ids_of(a[1], dev, "embedding");
@@ -149,7 +155,7 @@ PyObject* embedding(PyObject* const* a, Py_ssize_t n) {
     out = at::empty(shape, table.options().requires_grad(c10::nullopt));
   } else {
     int c;
-    out = elements(a[3], "embedding out", &c);
+    out = plain_elements(a[3], "embedding out", &c);
     if (c != code || out.device() != dev || !out.is_contiguous() || out.sizes() != at::IntArrayRef(shape))
       refuse(PyExc_ValueError, "embedding: out must be a contiguous ", table.scalar_type(), " tensor of shape ", at::IntArrayRef(shape), " on ", dev);
     apart(out, table, "embedding", "the table");
@@ -184,7 +190,7 @@ backward_args backward_of(PyObject* const* a, const char* who) {
   b.scale = (float)number(a[3]);
   b.padding = a[4] == Py_None ? -1 : integer(a[4]);
   // rows one element apart, any row stride (0 included), or a copy
-  b.g = g.dim() == 2 || b.n == 0 || b.width == 0 ? g : g.reshape({b.n, b.width});
+  b.g = (g.dim() == 2 || b.n == 0 || b.width == 0 ? g : g.reshape({b.n, b.width})).resolve_neg();
   if (b.n && b.width > 1 && b.g.stride(-1) != 1) b.g = b.g.contiguous();
   return b;
 }
@@ -220,7 +226,7 @@ PyObject* embedding_backward(PyObject* const* a, Py_ssize_t n) {
     type = type_of(a[7], b, who);
     out = at::empty({b.num_rows, b.width}, at::TensorOptions(b.dev).dtype(TYPES[type]));
   } else {
-    out = elements(a[5], "embedding_backward out", &type);
+    out = plain_elements(a[5], "embedding_backward out", &type);
     if (out.dim() != 2 || out.size(0) != b.num_rows || out.size(1) != b.width || out.device() != b.dev || (b.width > 1 && out.stride(1) != 1) ||
         (b.num_rows > 1 && out.stride(0) < b.width) || (type != b.code && type != ORCA_F32) || (a[7] != Py_None && type_of(a[7], b, who) != type))
       refuse(PyExc_ValueError, "embedding_backward: out must be a tensor of shape [", b.num_rows, ", ", b.width, "] on ", b.dev,
@@ -255,7 +261,7 @@ PyObject* embedding_backward_rows(PyObject* const* a, Py_ssize_t n) {
     for (int i = 0; i < 3; ++i)
       if (!THPVariable_Check(PyTuple_GET_ITEM(a[5], i))) refuse(PyExc_TypeError, who, ": out must hold tensors");
     ids = THPVariable_Unpack(PyTuple_GET_ITEM(a[5], 0));
-    rows = elements(PyTuple_GET_ITEM(a[5], 1), "embedding_backward_rows out", &type);
+    rows = plain_elements(PyTuple_GET_ITEM(a[5], 1), "embedding_backward_rows out", &type);
     count = THPVariable_Unpack(PyTuple_GET_ITEM(a[5], 2));
     if (ids.dim() != 1 || ids.size(0) != b.n || ids.scalar_type() != at::kLong || rows.dim() != 2 || rows.size(0) != b.n || rows.size(1) != b.width ||
         count.dim() != 1 || count.size(0) != 1 || count.scalar_type() != at::kInt || ids.device() != b.dev || rows.device() != b.dev ||
@@ -320,7 +326,7 @@ grad_arrays grads_of(PyObject* list, const char* who) {
     if (r.dev.index() < 0) r.dev = t.device();
     if (t.device() != r.dev) refuse(orca_error, who, ": the gradients must be on one HIP device");
     if (sparse) {
-      if (t.dim() != 2 || t.size(1) < 1 || t.size(1) > INT32_MAX || !t.is_contiguous() || count->scalar_type() != at::kInt || count->numel() != 1 ||
+      if (t.dim() != 2 || t.size(1) < 1 || t.size(1) > INT32_MAX || !t.is_contiguous() || t.is_neg() || count->scalar_type() != at::kInt || count->numel() != 1 ||
           count->device() != r.dev)
         refuse(PyExc_ValueError, who, ": a RowGrad needs contiguous [n, width] rows and an int32 count on their device");
       r.rows.resize(r.data.size() + 1, nullptr);
@@ -328,10 +334,10 @@ grad_arrays grads_of(PyObject* list, const char* who) {
       r.rows.back() = count->const_data_ptr<int32_t>();
       r.widths.back() = (int32_t)t.size(1);
     }
-    if (t.is_contiguous()) {
+    if (t.is_contiguous() && !t.is_neg()) {
       r.data.push_back(t.data_ptr());
     } else {
-      r.copies.emplace_back(t.contiguous(), r.data.size());
+      r.copies.emplace_back(t.contiguous().resolve_neg(), r.data.size());
       r.data.push_back(r.copies.back().first.data_ptr());
     }
     r.tensors.push_back(&t);
@@ -432,7 +438,7 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
       refuse(PyExc_ValueError, who, ": ", PyList_GET_SIZE(a[2]), " flat buffers for gradients of ", order.size(), " types");
     for (size_t k = 0; k < order.size(); ++k) {
       int code;
-      const at::Tensor& f = elements(PyList_GET_ITEM(a[2], k), "clip_grad_norm flat", &code);
+      const at::Tensor& f = plain_elements(PyList_GET_ITEM(a[2], k), "clip_grad_norm flat", &code);
       if (code != order[k] || f.numel() != need[code] || f.device() != g.dev || !f.is_contiguous())
         refuse(PyExc_ValueError, who, ": flat buffer ", k, " is not a contiguous ", TYPES[order[k]], " tensor of ", need[order[k]], " elements on ", g.dev);
       flat[code] = f.data_ptr();
