@@ -6,6 +6,7 @@
 // occurrences is spread over as many windows as it needs and two runs give the same bits.  (orca_scatter_add_flagged adds with
 // fp32 atomics in whatever order they arrive.)
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include "elem.h"
 
@@ -1189,12 +1190,21 @@ int key_bits(int64_t num_rows) {
   while ((num_rows >> bits) != 0) ++bits;
   return bits;
 }
+// A kernel's dynamic LDS is allowed once per device, and noted when that has happened: another thread's call (autograd runs a backward
+// pass on its own) does it again rather than launch ahead of it.
+int allow_lds(std::atomic<bool> (&done)[64], const void* kernel, int bytes) {
+  int dev = 0;
+  ORCA_HIP_TRY(hipGetDevice(&dev));
+  const bool known = dev >= 0 && dev < 64;
+  if (known && done[dev].load(std::memory_order_acquire)) return ORCA_OK;
+  ORCA_HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (known) done[dev].store(true, std::memory_order_release);
+  return ORCA_OK;
+}
 template <int THREADS, class TI, class TO, int VEC, bool ACCUMULATE>
 int launch_small(small_args a, hipStream_t stream) {
-  static bool seen[64] = {};
-  if (orca_first_use_on_device(seen))
-    ORCA_HIP_TRY(hipFuncSetAttribute((const void*)k_small<THREADS, TI, TO, VEC, ACCUMULATE>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                     small_layout(THREADS, THREADS * SMALL_ITEMS).bytes));
+  static std::atomic<bool> done[64];
+  if (int rc = allow_lds(done, (const void*)k_small<THREADS, TI, TO, VEC, ACCUMULATE>, small_layout(THREADS, THREADS * SMALL_ITEMS).bytes)) return rc;
   columns<TI>(&a);
   // workgroups: four ids, 16 KB of zeros or 65,536 rows each, at most one per CU (and one for each column block)
   int64_t want = ceil_div64(a.n, 4) * a.col_blocks;
@@ -1225,10 +1235,8 @@ range_work range_layout(char* ws, int64_t n, int64_t* bytes) {
   return w;
 }
 template <int THREADS> int launch_range_sort(const small_args& a, const range_work& w, int ranges, hipStream_t stream) {
-  static bool seen[64] = {};
-  if (orca_first_use_on_device(seen))
-    ORCA_HIP_TRY(hipFuncSetAttribute((const void*)k_range_sort<THREADS>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                     small_layout(THREADS, THREADS * SMALL_ITEMS).bytes));
+  static std::atomic<bool> done[64];
+  if (int rc = allow_lds(done, (const void*)k_range_sort<THREADS>, small_layout(THREADS, THREADS * SMALL_ITEMS).bytes)) return rc;
   k_range_sort<THREADS><<<(unsigned)ranges, THREADS, small_layout(THREADS, a.n).bytes, stream>>>(a, w);
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
