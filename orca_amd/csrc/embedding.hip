@@ -30,12 +30,15 @@ template <int VEC, class T, bool PAST = false> __device__ __forceinline__ void s
 }
 
 // Where accesses go past the caches, by the bytes they cover.  Measured with the pass that reads or writes them next to it (us, plain
-// -> past): lookup and a product over its output 17 MB 14.0 -> 13.3, 21 MB 16.0 -> 16.4, 128 MB 85 -> 94, 256 MB 192 -> 193, 512 MB
-// 372 -> 359 (the lookup alone 7.3 -> 5.6, .., 178 -> 149); dense gradient and the norm of it 256 MB 104 -> 112, 400 MB 164 -> 162,
-// 800 MB 318 -> 302; a product over grad_out and the gradient's pass over it 96 MB 70 -> 73, 128 MB 86.5 -> 85.8, 256 MB 156 -> 147.
-// In between, the 256 MB last-level cache hands the bytes to the neighbour.
+// -> past), since in between the 256 MB last-level cache hands the bytes to the neighbour:
+//   lookup (100 and 172 fp32, 512 and 2048 bf16) with a product, a row maximum, a matrix product and a layer norm over its output, geometric
+//     mean of past / plain: 0.25 to 2 MB 1.02 to 1.10, 4 to 8 MB 1.00 to 1.05, 12 MB 0.99 to 1.02, 18 MB 1.04 to 1.06, 200 MB 0.99 to 1.02, 256 MB
+//     0.98 to 1.01, 300 MB 0.96 to 1.00, 400 MB 0.96 to 0.99.  (The lookup by itself is faster past the caches from 4 MB on, 18 MB 8.7 -> 8.0,
+//     and its reader slower by more.)
+//   dense gradient and the norm of it: 256 MB 104 -> 112, 400 MB 164 -> 162, 800 MB 318 -> 302
+//   a product over grad_out and the gradient's pass over it: 96 MB 70 -> 73, 128 MB 86.5 -> 85.8, 256 MB 156 -> 147
 constexpr int64_t MB = 1000000;
-bool past_lookup(int64_t bytes) { return bytes <= 19 * MB || bytes >= 256 * MB; }
+bool past_lookup(int64_t bytes) { return bytes >= 256 * MB; }
 bool past_zeros(int64_t bytes) { return bytes >= 384 * MB; }
 bool past_gradient(int64_t bytes) { return bytes >= 128 * MB; }
 
