@@ -373,42 +373,69 @@ PyObject* grad_norm(PyObject* const* a, Py_ssize_t n) {
   return r;
 }
 
-// the bytes of the list's tensors, in their callers' storage: contiguous ones as they are, the others by their strides
-struct span {
-  const char *first, *last;           // from .. up to
-  const at::Tensor* strided;          // null: contiguous
-  region bytes() const { return strided ? region_of(*strided) : region{first, last - first, {}}; }
-};
-span span_of(const void* p, int64_t n, int code) { return {(const char*)p, (const char*)p + n * (code == ORCA_F32 ? 4 : 2), nullptr}; }
-std::vector<span> spans_of(const grad_arrays& g) {
-  std::vector<span> s;
-  s.reserve(g.data.size());
+// where a tensor's bytes begin and end in its caller's storage
+typedef std::pair<const char*, const char*> span;
+span span_of(const void* p, int64_t n, int code) { return {(const char*)p, (const char*)p + n * (code == ORCA_F32 ? 4 : 2)}; }
+// a list's tensors, the empty ones left out.  `strided`: those that are copied, by their strides (else null, and the span says it all)
+struct place { span s; const at::Tensor* strided; };
+std::vector<place> places_of(const grad_arrays& g) {
+  std::vector<place> r;
+  r.reserve(g.data.size());
   size_t next = 0;
   for (size_t i = 0; i < g.data.size(); ++i) {
     const bool copied = next < g.copies.size() && g.copies[next].second == i;
     next += copied;
     if (!g.sizes[i]) continue;
     if (copied) {
-      const region r = region_of(*g.tensors[i]);
-      s.push_back({r.p, r.end(), g.tensors[i]});
+      const region q = region_of(*g.tensors[i]);
+      r.push_back({{q.p, q.end()}, g.tensors[i]});
     } else {
-      s.push_back(span_of(g.data[i], g.sizes[i], g.types[i]));
+      r.push_back({span_of(g.data[i], g.sizes[i], g.types[i]), nullptr});
     }
   }
-  return s;
+  return r;
 }
-bool meet(const span& a, const span& b) {
-  return a.first < b.last && b.first < a.last && ((!a.strided && !b.strided) || meet(a.bytes(), b.bytes()));
+bool meet(const place& a, const place& b) {
+  auto bytes = [](const place& p) { return p.strided ? region_of(*p.strided) : region{p.s.first, p.s.second - p.s.first, {}}; };
+  return a.s.first < b.s.second && b.s.first < a.s.second && ((!a.strided && !b.strided) || meet(bytes(a), bytes(b)));
 }
+constexpr const char* TWICE = ": a tensor is in the list twice, or two of them overlap";
 void apart_in_list(std::vector<span> s, const char* who) {
-  std::sort(s.begin(), s.end(), [](const span& a, const span& b) { return a.first < b.first; });
-  std::vector<const span*> open;                // those that reach past the beginning of the next one
-  for (const span& x : s) {
-    open.erase(std::remove_if(open.begin(), open.end(), [&](const span* o) { return o->last <= x.first; }), open.end());
-    for (const span* o : open)
-      if (meet(*o, x)) refuse(PyExc_ValueError, who, ": a tensor is in the list twice, or two of them overlap");
+  if (!std::is_sorted(s.begin(), s.end())) std::sort(s.begin(), s.end());
+  for (size_t i = 1; i < s.size(); ++i)
+    if (s[i].first < s[i - 1].second) refuse(PyExc_ValueError, who, TWICE);
+}
+void apart_in_list(const grad_arrays& g, const char* who) {
+  if (g.copies.empty()) {
+    std::vector<span> s;
+    s.reserve(g.data.size());
+    for (size_t i = 0; i < g.data.size(); ++i)
+      if (g.sizes[i]) s.push_back(span_of(g.data[i], g.sizes[i], g.types[i]));
+    return apart_in_list(std::move(s), who);
+  }
+  std::vector<place> all = places_of(g);
+  std::sort(all.begin(), all.end(), [](const place& a, const place& b) { return a.s < b.s; });
+  std::vector<const place*> open;               // those that reach past the beginning of the next one
+  for (const place& x : all) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const place* o) { return o->s.second <= x.s.first; }), open.end());
+    for (const place* o : open)
+      if (meet(*o, x)) refuse(PyExc_ValueError, who, TWICE);
     open.push_back(&x);
   }
+}
+void apart_from_list(const std::vector<span>& flat, const grad_arrays& g, const char* who) {
+  constexpr const char* text = ": a flat buffer overlaps a gradient";
+  if (g.copies.empty()) {
+    for (size_t i = 0; i < g.data.size(); ++i) {
+      const span r = span_of(g.data[i], g.sizes[i], g.types[i]);
+      for (const span& f : flat)
+        if (f.first < r.second && r.first < f.second && g.sizes[i]) refuse(PyExc_ValueError, who, text);
+    }
+    return;
+  }
+  for (const place& r : places_of(g))
+    for (const span& f : flat)
+      if (meet(place{f, nullptr}, r)) refuse(PyExc_ValueError, who, text);
 }
 
 // clip_grad_norm(list, max_norm, flat buffers or None) -> norm
@@ -420,7 +447,7 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
   const c10::DeviceGuard guard(g.dev);
   void* flat[3] = {nullptr, nullptr, nullptr};
   if (a[2] == Py_None) {
-    apart_in_list(spans_of(g), who);
+    apart_in_list(g, who);
     for (const auto& c : g.copies)
       for (int64_t d = 0; d < g.tensors[c.second]->dim(); ++d)
         if (g.tensors[c.second]->stride(d) == 0 && g.tensors[c.second]->size(d) > 1) refuse(PyExc_ValueError, who, ": an expanded tensor cannot be clipped in place");
@@ -428,7 +455,7 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
     if (!PyList_Check(a[2])) refuse(PyExc_TypeError, who, ": flat must be a list of tensors");
     std::vector<int> order;                       // the types as they first appear
     int64_t need[3] = {0, 0, 0};
-    std::vector<span> written;
+    std::vector<span> outputs;
     for (size_t i = 0; i < g.data.size(); ++i) {
       const int t = g.types[i];
       if (std::find(order.begin(), order.end(), t) == order.end()) order.push_back(t);
@@ -442,12 +469,10 @@ PyObject* clip_grad_norm(PyObject* const* a, Py_ssize_t n) {
       if (code != order[k] || f.numel() != need[code] || f.device() != g.dev || !f.is_contiguous())
         refuse(PyExc_ValueError, who, ": flat buffer ", k, " is not a contiguous ", TYPES[order[k]], " tensor of ", need[order[k]], " elements on ", g.dev);
       flat[code] = f.data_ptr();
-      if (f.numel()) written.push_back(span_of(f.data_ptr(), f.numel(), code));
+      if (f.numel()) outputs.push_back(span_of(f.data_ptr(), f.numel(), code));
     }
-    for (const span& r : spans_of(g))
-      for (const span& w : written)
-        if (meet(w, r)) refuse(PyExc_ValueError, who, ": a flat buffer overlaps a gradient");
-    apart_in_list(std::move(written), who);
+    apart_from_list(outputs, g, who);
+    apart_in_list(std::move(outputs), who);
   }
   const auto opt = at::TensorOptions(g.dev).dtype(at::kFloat);
   const at::Tensor norm = at::empty({}, opt), ws = at::empty({grad_norm_workspace_bytes()}, opt.dtype(at::kByte));

@@ -22,6 +22,7 @@ from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import ops
 from ._lib import ORCA_D as D
@@ -249,6 +250,11 @@ _table.impl("embedding", _embedding, "CompositeExplicitAutograd")
 _table.impl("embedding_backward", _embedding_backward, "CompositeExplicitAutograd")
 
 
+def _no_tangent(x, name):
+  if forward_ad.unpack_dual(x).tangent is not None:
+    raise NotImplementedError(f"orca::{name} has no forward-mode derivative")
+
+
 class _Embedding(torch.autograd.Function):
   @staticmethod
   def forward(ctx, table, ids, scale, padding_idx):
@@ -260,7 +266,12 @@ class _Embedding(torch.autograd.Function):
   @staticmethod
   def backward(ctx, g_out):
     ids, = ctx.saved_tensors
-    return torch.ops.orca.embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx), None, None, None
+    if torch.is_grad_enabled():         # (create_graph)
+      grad = torch.ops.orca.embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx)
+    else:
+      _no_tangent(g_out, "embedding_backward")
+      grad = _embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx)
+    return grad, None, None, None
 
 
 class _EmbeddingBackward(torch.autograd.Function):
@@ -280,13 +291,14 @@ class _EmbeddingBackward(torch.autograd.Function):
 
 
 def _table_autograd(name, function):
+  op = getattr(torch.ops.orca, name).default
+
   def kernel(x, *args):
-    if torch.autograd.forward_ad.unpack_dual(x).tangent is not None:
-      raise NotImplementedError(f"orca::{name} has no forward-mode derivative")
+    _no_tangent(x, name)
     if torch.is_grad_enabled() and x.requires_grad:
       return function.apply(x, *args)
     with torch._C._AutoDispatchBelowAutograd():
-      return getattr(torch.ops.orca, name)(x, *args)
+      return op(x, *args)
   _table.impl(name, kernel, "Autograd")
 
 
