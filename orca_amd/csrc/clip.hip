@@ -3,9 +3,9 @@
 // No atomics and no host read.  Short lists, two launches: k_norm_partial leaves one fp64 sum per workgroup, and every workgroup of k_clip
 // adds those sums up in the same order (while its first piece is on its way) before it scales its share.  Long ones, where that time
 // shows: k_norm_finish adds them up in between, and a workgroup of k_clip takes a piece or four and ends.  Squares and sums are fp64:
-// neither overflows nor vanishes for any fp32 input, and the conversions hide behind the loads (4.5 elements per clock and CU at the
-// HBM rate for 16-bit gradients).  Bound by the HBM: 400 million elements in 300 tensors, 580 MB, 425 us = 138 (4.2 TB/s) + 5 + 282 (4.1
-// TB/s); short lists by the two launches: 35 tensors of 2.9 MB 3.5 + 4.6 us.
+// neither overflows nor vanishes for any fp32 input, and the conversions hide behind the loads (5 elements per clock and CU at the
+// HBM rate for 16-bit gradients).  Bound by the HBM: 400 million elements in 300 tensors, 871 MB, 425 us = 138 (6.3 TB/s) + 5 + 282 (6.2
+// TB/s; torch's copy of 1 GiB runs at 5.0); short lists by the two launches: 35 tensors of 2.9 MB 3.5 + 4.6 us.
 //   A list travels in the kernel's arguments, under 4 KB: 12 bytes per tensor (16 with flat buffers), so that a few hundred tensors
 // are one launch.  With a search by scalar loads through 41 bytes per tensor, k_norm_partial took 6.4 us for 32 tensors of 2.9 MB.
 #include <algorithm>
@@ -17,10 +17,11 @@ constexpr int PIECE = 16384, SMALL_PIECE = 4096, LONG_PIECE = 8192;
 // From here on a list is long, us for fp32 and both ways: into flat buffers 80 MB 41.0 (long: 45.6), 100 MB 54.9 (54.5), 120 MB 72.0 (63.2),
 // 500 MB 286 (246); in place 120 MB 55.6 (62.9), 160 MB 80.9 (80.1), 240 MB 133 (115), 1 GB 545 (466).
 constexpr int64_t LONG_FLAT = 100000000, LONG_IN_PLACE = 160000000;
-// The products of long lists are written past the caches (non-temporal; 580 MB in 16 bits, flat: 425, with plain stores 502) and their
-// gradients read so by k_clip (439 with plain loads), by k_norm_partial from here on: below, the last-level cache keeps some of them for
-// k_clip (flat, plain and past: 240 MB 111 and 117, 500 MB 239 and 246, 580 MB 430 and 425, 1 GB 495 and 492).
-constexpr int64_t PAST_NORM = 540000000;
+// The products of long lists are written past the caches (non-temporal; 871 MB, most of it in 16 bits, flat: 425, with plain stores 502)
+// and their gradients read so by k_clip (439 with plain loads), by k_norm_partial from here on: below, the last-level cache keeps some of
+// them for k_clip (300 tensors of both widths, flat, plain and past: 120 MB 69.8 and 73.6, 300 MB 147 and 156, 500 MB 245 and 251, 600 MB 295
+// and 296, 700 MB 346 and 341, 800 MB 398 and 391, 1 GB 500 and 487; all fp32 500 MB 241 and 247, 700 MB 343 and 344, 800 MB 394 and 393).
+constexpr int64_t PAST_NORM = 650000000;
 // Workgroups of a launch of k_norm_partial, and the most partial sums of a call.
 constexpr int GRID = 2048, LONG_GRID = 1024, PARTS = 2048, LONG_PARTS = 8192;
 // Pieces of a workgroup of k_clip on a long list in place: when the coefficient is 1 they all only come and go (500 MB of fp32 with one
