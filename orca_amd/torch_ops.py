@@ -231,8 +231,8 @@ _lib.register_autograd("orca::history_pull_pushed", _hpp_backward, setup_context
 # order.  They are defined with their own autograd kernels: what custom_op registers lets the tangent of a table that does not
 # require a gradient go without a word.
 _table = _lib.Library("orca", "FRAGMENT")
-_table.define("embedding(Tensor table, Tensor ids, float scale, int padding_idx) -> Tensor")
-_table.define("embedding_backward(Tensor grad_out, Tensor ids, int num_rows, float scale, int padding_idx) -> Tensor")
+_table.define("embedding(Tensor table, Tensor ids, float scale, SymInt padding_idx) -> Tensor")
+_table.define("embedding_backward(Tensor grad_out, Tensor ids, SymInt num_rows, float scale, SymInt padding_idx) -> Tensor")
 
 
 def _embedding(table, ids, scale, padding_idx):
@@ -266,12 +266,7 @@ class _Embedding(torch.autograd.Function):
   @staticmethod
   def backward(ctx, g_out):
     ids, = ctx.saved_tensors
-    if torch.is_grad_enabled():         # (create_graph)
-      grad = torch.ops.orca.embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx)
-    else:
-      _no_tangent(g_out, "embedding_backward")
-      grad = _embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx)
-    return grad, None, None, None
+    return torch.ops.orca.embedding_backward(g_out, ids, ctx.num_rows, ctx.scale, ctx.padding_idx), None, None, None
 
 
 class _EmbeddingBackward(torch.autograd.Function):
@@ -304,6 +299,7 @@ def _table_autograd(name, function):
 
 _table_autograd("embedding", _Embedding)
 _table_autograd("embedding_backward", _EmbeddingBackward)
+embedding, embedding_backward = torch.ops.orca.embedding, torch.ops.orca.embedding_backward
 
 
 OPS = ("sample_recent", "sample_uniform", "tgat_dense", "tgat_gather", "gru_cell", "message_store", "history_push",

@@ -106,3 +106,12 @@ def test_second_derivative_of_the_kernels(padding, wide):
   size = penalty(plain, table.detach().cpu().double().abs().requires_grad_(), weight.cpu().double().abs(), IDS, 0.5, padding)
   for a, b, s in zip(got, want, size):
     assert bool(((a.cpu().double() - b).abs() <= 24 * u * s).all())
+
+
+def test_the_module_offers_the_ops(stand_ins):
+  """as torch_ops.tgat_gather and the others; symbolic sizes pass through the schema"""
+  table = torch.randn(V, W, requires_grad=True)
+  out = torch_ops.embedding(table, IDS, 2.0, -1)
+  grad, = torch.autograd.grad(out.sum(), table, retain_graph=True)
+  assert torch.equal(out, table[IDS] * 2) and torch.equal(grad, torch_ops.embedding_backward(torch.ones(2, 3, W), IDS, V, 2.0, -1))
+  assert str(torch.ops.orca.embedding.default._schema) == "orca::embedding(Tensor table, Tensor ids, float scale, SymInt padding_idx) -> Tensor"
