@@ -248,6 +248,9 @@ def _embedding_backward(grad_out, ids, num_rows, scale, padding_idx):
 
 _table.impl("embedding", _embedding, "CompositeExplicitAutograd")
 _table.impl("embedding_backward", _embedding_backward, "CompositeExplicitAutograd")
+# (what tracing runs instead: shapes and types)
+_lib.register_fake("orca::embedding", lambda table, ids, scale, padding_idx: table.new_empty((*ids.shape, table.shape[1])))
+_lib.register_fake("orca::embedding_backward", lambda grad_out, ids, num_rows, scale, padding_idx: grad_out.new_empty((num_rows, grad_out.shape[-1])))
 
 
 def _no_tangent(x, name):

@@ -115,3 +115,17 @@ def test_the_module_offers_the_ops(stand_ins):
   grad, = torch.autograd.grad(out.sum(), table, retain_graph=True)
   assert torch.equal(out, table[IDS] * 2) and torch.equal(grad, torch_ops.embedding_backward(torch.ones(2, 3, W), IDS, V, 2.0, -1))
   assert str(torch.ops.orca.embedding.default._schema) == "orca::embedding(Tensor table, Tensor ids, float scale, SymInt padding_idx) -> Tensor"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tracing(dtype):
+  """shapes and types without data, through the derivative too; no kernel and no stand-in is called"""
+  from torch._subclasses.fake_tensor import FakeTensorMode
+  with FakeTensorMode():
+    table = torch.empty(V, W, dtype=dtype, requires_grad=True)
+    out = torch.ops.orca.embedding(table, torch.zeros(2, 3, dtype=torch.int32), 0.5, 0)
+    assert out.shape == (2, 3, W) and out.dtype == dtype
+    grad, = torch.autograd.grad(out.sum(), table, retain_graph=True)
+    assert grad.shape == (V, W) and grad.dtype == dtype
+    again, = torch.autograd.grad((out.square().sum()), table, create_graph=True)
+    assert torch.autograd.grad(again.sum(), table)[0].shape == (V, W)
