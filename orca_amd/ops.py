@@ -665,8 +665,8 @@ class FusedAdam:
     self._state = torch.zeros(2, max(n, 1), dtype=torch.float32, device=dev)     # exp_avg | exp_avg_sq, one fill
     self.exp_avg, self.exp_avg_sq, o = {}, {}, 0
     for k, v in self.params.items():
-      if v.dtype != torch.float32 or not v.is_contiguous() or not v.is_cuda:
-        raise _lib.OrcaError(f"FusedAdam: parameter {k} must be a contiguous fp32 tensor on the HIP device")
+      if v.dtype != torch.float32 or not v.is_contiguous() or not v.is_cuda or v.device != dev:
+        raise _lib.OrcaError(f"FusedAdam: parameter {k} must be a contiguous fp32 tensor on the HIP device (one for all of them)")
       self.exp_avg[k] = self._state[0, o:o + v.numel()]
       self.exp_avg_sq[k] = self._state[1, o:o + v.numel()]
       o += -(-v.numel() // 64) * 64
@@ -687,7 +687,7 @@ class FusedAdam:
           raise _lib.OrcaError(f"FusedAdam: row gradient of {k} does not match its parameter")
         used[k] = g
       else:
-        if g.numel() != p.numel() or g.dtype != torch.float32 or not g.is_cuda:
+        if g.numel() != p.numel() or g.dtype != torch.float32 or g.device != p.device:
           raise _lib.OrcaError(f"FusedAdam: gradient of {k} does not match its parameter")
         used[k] = g.contiguous()
     norm = coef = None
