@@ -12,12 +12,9 @@ OUT = os.path.join(HERE, "liborca_hip.so")
 HOST = os.path.join(HERE, "_host.so")      # csrc/bind.cpp: torch tensors -> C ABI for the calls where the host's time counts
 SOURCES = ["csr.hip", "tgat.hip", "tgat_bwd.hip", "gru_bwd.hip", "gru.hip", "state.hip", "plan.hip", "plan_dev.hip", "engine.hip", "optim.hip", "clip.hip", "clip_adam.hip", "embedding.hip", "decoder.hip"]
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-Wall",
-         "-Wno-unused-result", "-Wno-unused-function"]
-
-
-# no packed fp32 instructions in the sources that carry this (some of their forms have given wrong results on gfx950)
-NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SCALAR_FP32 = {"clip.hip", "clip_adam.hip", "embedding.hip"}
+         "-Wno-unused-result", "-Wno-unused-function",
+         # no packed fp32 instructions: some of their forms have given wrong results on gfx950, now and then and without an error
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(target, deps):
@@ -39,8 +36,8 @@ def build(force=False, verbose=False):
     src = os.path.join(CSRC, s)
     obj = os.path.join(CSRC, "build", s.replace(".hip", ".o"))
     objs.append(obj)
-    if force or _stale(obj, [src] + headers):
-      jobs.append([hipcc] + FLAGS + (NO_PACKED if s in SCALAR_FP32 else []) + ["-c", src, "-o", obj])
+    if force or _stale(obj, [src, os.path.abspath(__file__)] + headers):      # (this file: the flags)
+      jobs.append([hipcc] + FLAGS + ["-c", src, "-o", obj])
 
   def run(cmd):
     if verbose:

@@ -48,3 +48,13 @@ int adam_groups(int n, float* const* params, const float* const* grads, float* c
   ORCA_LAUNCH_CHECK();
   return ORCA_OK;
 }
+
+// One element of the step.  Which products are fused with their sums is written out: the compiler's choice changes with its flags.
+__device__ __forceinline__ void adam_element(float gi, float* p, float* m, float* v, const AdamScalars& k) {
+#pragma clang fp contract(off)
+  const float mi = fmaf(k.w1, gi - *m, *m);
+  const float vi = *v * k.b2 + k.w2 * gi * gi;
+  *m = mi;
+  *v = vi;
+  *p = fmaf(-k.step_size, mi / (sqrtf(vi) / k.bc2_sqrt + k.eps), *p);
+}

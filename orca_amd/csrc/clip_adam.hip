@@ -1,19 +1,10 @@
 // Adam steps that k_adam (optim.hip) has no form for: with the gradients scaled by a device value on the way (the clipping coefficient of
 // orca_grad_norm: no pass of its own over the gradients, no host read), and for the rows of a row-sparse gradient.
 //   m += (1 - b1) (g - m);  v = b2 v + (1 - b2) g g;  p -= (lr / (1 - b1^t)) * m / (sqrt(v) / sqrt(1 - b2^t) + eps),   g = s * gradient
-// The products are fused with the sums exactly where k_adam's are, so that a coefficient of 1 gives k_adam's bits.
+// The arithmetic is k_adam's (adam.h), so that a coefficient of 1 gives k_adam's bits.
 #include "adam.h"
 
 namespace {
-__device__ __forceinline__ void adam_element(float gi, float* p, float* m, float* v, const AdamScalars& k) {
-#pragma clang fp contract(off)
-  const float mi = fmaf(k.w1, gi - *m, *m);
-  const float vi = *v * k.b2 + k.w2 * gi * gi;
-  *m = mi;
-  *v = vi;
-  *p = fmaf(-k.step_size, mi / (sqrtf(vi) / k.bc2_sqrt + k.eps), *p);
-}
-
 __global__ __launch_bounds__(256) void k_adam_scaled(AdamGroup grp, AdamScalars k, const float* __restrict__ scale) {
   int t = 0;
 #pragma unroll

@@ -6,8 +6,7 @@
 #include "adam.h"
 
 namespace {
-__global__ __launch_bounds__(256) void k_adam(AdamGroup grp, float w1, float b2, float w2, float step_size, float bc2_sqrt,
-                                              float eps) {
+__global__ __launch_bounds__(256) void k_adam(AdamGroup grp, AdamScalars k) {
   int t = 0;
 #pragma unroll
   for (int i = 1; i < ADAM_MAX; ++i) t += (i < grp.n && (int)blockIdx.x >= grp.first[i]) ? 1 : 0;
@@ -21,13 +20,7 @@ __global__ __launch_bounds__(256) void k_adam(AdamGroup grp, float w1, float b2,
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int64_t i = base + 256 * u;
-    if (i >= n) continue;
-    const float gi = g[i];
-    const float mi = m[i] + w1 * (gi - m[i]);
-    const float vi = v[i] * b2 + w2 * gi * gi;
-    m[i] = mi;
-    v[i] = vi;
-    p[i] -= step_size * (mi / (sqrtf(vi) / bc2_sqrt + eps));
+    if (i < n) adam_element(g[i], p + i, m + i, v + i, k);
   }
 }
 }  // namespace
@@ -37,6 +30,6 @@ ORCA_API int orca_adam_step(int n, float* const* params, const float* const* gra
                             int64_t step, void* stream) {
   const AdamScalars k = adam_scalars(lr, beta1, beta2, eps, step < 1 ? 1 : step);
   return adam_groups(n, params, grads, exp_avg, exp_avg_sq, sizes, step, [&](const AdamGroup& grp, unsigned blocks) {
-    k_adam<<<blocks, 256, 0, (hipStream_t)stream>>>(grp, k.w1, k.b2, k.w2, k.step_size, k.bc2_sqrt, k.eps);
+    k_adam<<<blocks, 256, 0, (hipStream_t)stream>>>(grp, k);
   });
 }

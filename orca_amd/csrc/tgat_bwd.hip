@@ -310,7 +310,9 @@ __device__ __forceinline__ void wgrad_tile(const GemmArgs& g, int m0, int n0, in
     o.b = *reinterpret_cast<const f32x4*>(bp + (int64_t)kc * g.sbk);
     return o;
   };
+  // (Product and sum stay apart -- exact either way: fused, the launch of 1080 workgroups took 57 us instead of 42.)
   auto mask = [&](Ops& o, int k0) {
+#pragma clang fp contract(off)
     const float kokf = k0 + kq < ke ? 1.f : 0.f;
 #pragma unroll
     for (int t = 0; t < V; ++t) o.a[t] *= kokf;

@@ -6,7 +6,7 @@ set -e
 cd "$(dirname "$0")/.."
 python -m orca_amd.build > /dev/null
 cd orca_amd/csrc
-/opt/rocm/bin/hipcc -O3 --offload-arch=gfx950 -std=c++20 -fPIC -fvisibility=hidden -I../../include -DORCA_WAVE_STAMPS \
+/opt/rocm/bin/hipcc -O3 --offload-arch=gfx950 -std=c++20 -fPIC -fvisibility=hidden -Xclang -target-feature -Xclang -packed-fp32-ops -I../../include -DORCA_WAVE_STAMPS \
   -c tgat.hip -o build/tgat_diag.o
 objs=$(ls build/*.o | grep -v -e tgat_diag.o -e '/tgat.o')
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ../liborca_hip_diag.so $objs build/tgat_diag.o
