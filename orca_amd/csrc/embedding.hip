@@ -49,8 +49,8 @@ bool fits_launch(int64_t blocks, int threads) { return blocks * threads < (1LL <
 // ---- lookup ----------------------------------------------------------------------------------------------------------
 // The output is a list of n * C chunks of 16 bytes; the last chunk of a row starts at width - VEC, so that every access is
 // whole (it overlaps the one before it: both write the same values).  Rows narrower than a chunk go element by element.
-// Bound by the id -> row latency of one round of workgroups (45,045 rows of 100 fp32: 6.2 us, 4.0 TB/s), large ones by the HBM (65,536 rows
-// of 2048 bf16: 59.7 us, 5.8 TB/s: repeated rows come out of the caches); small ones by the launch (600 rows: 3.1 us).
+// Bound by the id -> row latency of one round of workgroups (45,045 rows of 100 fp32: 7.2 us, 3.5 TB/s), large ones by the HBM (65,536 rows
+// of 2048 bf16: 59.8 us, 5.8 TB/s: repeated rows come out of the caches); small ones by the launch (600 rows: 3.2 us).
 constexpr int LOOK_U = 4;                 // chunks per thread: that many independent id -> row chains
 template <class T, int VEC, bool PAST, class I>
 __global__ __launch_bounds__(256) void k_embedding(const T* __restrict__ table, int64_t n_rows, int64_t ld,
@@ -201,7 +201,8 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_count(sort_src src, int s
   for (int b = threadIdx.x; b < bins; b += SORT_THREADS) counts[(int64_t)blockIdx.x * bins + b] = h[b];
 }
 
-// counts[tile][bin] -> the number in the tiles before; totals[bin]
+// counts[tile][bin] -> the number in the tiles before; totals[bin].  Bound by its round trips, eight tiles in each (a million pairs, 489
+// tiles: 34 us a pass; four million: 136).
 __global__ __launch_bounds__(64) void k_sort_columns(uint32_t* __restrict__ counts, int64_t tiles, int bins, uint32_t* __restrict__ totals) {
   const int b = blockIdx.x * 64 + threadIdx.x;
   if (b >= bins) return;
