@@ -107,6 +107,14 @@ region region_of(const at::Tensor& t) {
     r.run += r.outer.front().first * (r.outer.front().second - 1);
     r.outer.erase(r.outer.begin());
   }
+  for (size_t d = 1; d < r.outer.size();) {       // (a dimension that goes on where the one before ends)
+    auto& before = r.outer[d - 1];
+    if (r.outer[d].first != before.first * before.second) ++d;
+    else {
+      before.second *= r.outer[d].second;
+      r.outer.erase(r.outer.begin() + d);
+    }
+  }
   return r;
 }
 // Whether they share a byte.  Views that interleave (column blocks of one matrix) do not.
