@@ -129,3 +129,11 @@ def test_tracing(dtype):
     assert grad.shape == (V, W) and grad.dtype == dtype
     again, = torch.autograd.grad((out.square().sum()), table, create_graph=True)
     assert torch.autograd.grad(again.sum(), table)[0].shape == (V, W)
+
+
+@pytest.mark.parametrize("padding", [-1, 3])
+def test_registrations(stand_ins, padding):
+  """torch's own check of an op's schema, derivative, tracing and compiled backward"""
+  table = torch.randn(V, W, requires_grad=True)
+  torch.library.opcheck(torch.ops.orca.embedding.default, (table, IDS, 0.5, padding))
+  torch.library.opcheck(torch.ops.orca.embedding_backward.default, (torch.randn(2, 3, W, requires_grad=True), IDS, V, 0.5, padding))
