@@ -655,7 +655,8 @@ class FusedAdam:
   """torch.optim.Adam(params, lr) (train.py:180) as one launch per step (orca_adam_step): params is a dict name ->
   fp32 device tensor, updated in place; step(grads) takes a dict with (a subset of) the same names -- a parameter
   without a gradient is skipped, as torch skips p.grad is None.  A RowGrad (fp32 rows) as a gradient updates its rows only: the
-  others and their moments stay as they are, as with torch.optim.SparseAdam."""
+  others and their moments stay as they are, as with torch.optim.SparseAdam.  A step counts as an in-place change of the tensors that
+  were passed and of those that share their version (a Parameter itself or its detach(); its .data has a version of its own)."""
 
   def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8):
     self.params = {k: v for k, v in params.items()}
@@ -709,6 +710,8 @@ class FusedAdam:
         sizes = (ctypes.c_int64 * n)(*[x[0].numel() for x in lst])
         check(_lib.load().orca_adam_step_scaled(n, arr(0), arr(1), arr(2), arr(3), sizes, self.lr, self.betas[0], self.betas[1],
                                                 self.eps, t, ptr(coef), stream()), "orca_adam_step")
+    # written by address: whoever keeps something made from a parameter (a layer its packed weights, autograd its saved values) asks its version
+    torch.autograd.graph.increment_version([self.params[k] for k in used])
     return norm
 
 
