@@ -1,5 +1,5 @@
-"""FusedAdam's launches run on its parameters' device: tensors of another one are refused (a stand-in says where it lies: a box may hold
-one GPU)."""
+"""FusedAdam's launches run on its parameters' device: tensors of another one are refused (a stand-in says where it lies: one GPU
+is enough)."""
 import pytest
 import torch
 
