@@ -1,5 +1,5 @@
 """Builds liborca_hip.so (the C-ABI library declared in include/orca_hip.h) in-tree with hipcc for
-gfx950.  Run here on the CPU container (hipcc cross-compiles); the .so travels to the GPU box."""
+gfx950.  Needs no GPU (hipcc cross-compiles); the .so files lie beside the sources."""
 import os
 import subprocess
 import sys
